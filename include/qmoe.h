@@ -34,7 +34,8 @@ extern "C" {
 enum qmoe_type {
     QMOE_TYPE_F32  = 0,
     QMOE_TYPE_Q4_0 = 2,
-    QMOE_TYPE_Q8_0 = 8
+    QMOE_TYPE_Q8_0 = 8,
+    QMOE_TYPE_BF16 = 30  /* rows of the operators below the layer (qmoe_fp8_* and on) */
 };
 
 enum qmoe_status {
@@ -331,6 +332,106 @@ int qmoe_rms_norm(const float* x, const float* w, int32_t n_tokens, int32_t n_em
  * skipped), i.e. ((r0+r1)+(r2+r3))+((r4+r5)+(r6+r7)).  No counterpart in the
  * reference (it sums inside ggml_rms_norm); the input of forward_norm_chain. */
 int qmoe_rms_partials(const float* x, int32_t n_tokens, int32_t n_embd, double* out, void* hip_stream);
+
+/* ---------------------------------------------------------------------------
+ * The feed-forward in 8-bit floats, as operators: for expert weights that come
+ * as e4m3 with one f32 scale per block of 128 x 128 (a layer above takes
+ * Q4_0/Q8_0).  One block of the model is
+ *   qmoe_residual_norm -> (router) -> qmoe_sort_tokens -> qmoe_fp8_matmul (gate
+ *   and up, rows read through the token list) -> qmoe_fp8_quantize (SwiGLU) ->
+ *   qmoe_fp8_matmul (down) -> qmoe_combine_tokens -> the next qmoe_residual_norm.
+ * No counterpart in the reference (its experts are GGUF blocks).  e4m3 is the OCP
+ * type (largest value 448, no infinities).  Rows are packed; x_type is
+ * QMOE_TYPE_F32 or QMOE_TYPE_BF16.  No call allocates, synchronises or keeps
+ * anything: all may be captured into a graph.  Index arrays are read on the
+ * device: values outside their range are ignored as each call says, never
+ * followed.  Zero rows are a no-op.
+ * ------------------------------------------------------------------------- */
+enum qmoe_fp8_act {
+    QMOE_FP8_ACT_NONE   = 0,
+    QMOE_FP8_ACT_SWIGLU = 1,  /* v = g / (1 + exp(-g)) * u */
+    QMOE_FP8_ACT_GEGLU  = 2   /* v = gelu(g) * u, the tanh form, in f32 */
+};
+/* q[n_rows][n_cols] (e4m3) and scale[n_rows][ceil(n_cols/128)] of v: x itself,
+ * or the activation of x's two halves (x is then [n_rows][2 n_cols], gate columns
+ * first).  Per block of 128 columns (the last may be shorter) m = the largest |v|,
+ * at least 1e-30: scale = m / 448, q = e4m3(v * f32(448 / m)), ties to even.  A
+ * block with a NaN has a NaN scale; one with an infinity an infinite scale. */
+int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_cols, int32_t act,
+                      uint8_t* q, float* scale, void* hip_stream);
+
+/* y[r][j] = sum_b a_scale[s][b] w_scale[e][j/128][b] sum_{i in block b} a[s][i] w[e][j][i]
+ * (y_type f32 or bf16; every sum in f32):
+ *   a [a_rows][k] e4m3, a_scale [a_rows][ceil(k/128)];
+ *   w [n_experts][n][k] e4m3, w_scale [n_experts][ceil(n/128)][ceil(k/128)];
+ *   offsets NULL: n_experts is 1 and every row uses the one matrix; else
+ *     offsets[n_experts + 1], rising: row r uses the expert e with offsets[e] <= r <
+ *     offsets[e+1] (values outside [0, n_rows] count as its ends); rows before
+ *     offsets[0] or from offsets[n_experts] on are left as they were;
+ *   rows NULL: s = r (n_rows == a_rows); else s = rows[r], and a row with s outside
+ *     [0, a_rows) is zeros.
+ * k is a multiple of 16; a and w are 16-byte aligned.  y overlaps no input. */
+int qmoe_fp8_matmul(const uint8_t* a, const float* a_scale, int32_t a_rows, const uint8_t* w, const float* w_scale,
+                    int32_t n_experts, int32_t n, int32_t k, const int32_t* offsets, const int32_t* rows,
+                    int32_t n_rows, void* y, int32_t y_type, void* hip_stream);
+
+/* The lists of a routing topk_idx[n_tokens][top_k] (assignment a = t * top_k + j):
+ *   offsets[n_experts+1]  each expert's first row, and the number of rows;
+ *   rows[n_tokens*top_k]  assignments grouped by expert, ascending within one;
+ *   tokens[...]           their tokens, rows[i] / top_k;
+ *   place[n_tokens][top_k] each assignment's index in rows.
+ * An id outside [0, n_experts) drops its assignment: place -1; rows and tokens
+ * are -1 from offsets[n_experts] on.  n_experts <= 1024, top_k <= 64.  No tokens:
+ * the offsets (zeros) are still written. */
+int qmoe_sort_tokens(const int32_t* topk_idx, int32_t n_tokens, int32_t top_k, int32_t n_experts,
+                     int32_t* offsets, int32_t* rows, int32_t* tokens, int32_t* place, void* hip_stream);
+/* y[place[t][j]] = x[t], elements of elem_bytes (1, 2 or 4): the rows in the
+ * experts' order; rows from offsets[n_experts] on are zeros.  Its gradient is
+ * qmoe_combine_tokens with w and residual NULL. */
+int qmoe_gather_tokens(const void* x, int32_t elem_bytes, int32_t n_tokens, int32_t n_cols, int32_t top_k,
+                       int32_t n_experts, const int32_t* offsets, const int32_t* place, void* y, void* hip_stream);
+/* y[t] = residual[t] + sum_j w[t][j] ys[place[t][j]], j in order in f32, rounded
+ * once; w NULL: ones; residual NULL: zeros, else y may be it.  A place outside
+ * [0, n_tokens*top_k) adds nothing. */
+int qmoe_combine_tokens(const void* ys, int32_t x_type, int32_t n_tokens, int32_t n_cols, int32_t top_k,
+                        const int32_t* place, const float* w, const void* residual, void* y, void* hip_stream);
+/* Gradients of qmoe_combine_tokens (the residual's is dy): dys[place[t][j]] =
+ * w[t][j] dy[t], dw[t][j] = <dy[t], ys[place[t][j]]> in f32; a dropped assignment's
+ * dw is 0, rows of dys from offsets[n_experts] on are zeros.  Both are the same
+ * bits on every run. */
+int qmoe_combine_tokens_backward(const void* dy, const void* ys, int32_t x_type, int32_t n_tokens, int32_t n_cols,
+                                 int32_t top_k, int32_t n_experts, const int32_t* offsets, const int32_t* place,
+                                 const float* w, void* dys, float* dw, void* hip_stream);
+
+/* The norms between two blocks in one pass over [n_tokens][n_embd] rows (n_embd <= 16384):
+ *   u  = y / sqrt(mean(y^2) + eps) * post_w   (post_w NULL: u = y)
+ *   u  = u * sigmoid(gate) or u * silu(gate)  (gate NULL: not)
+ *   x' = x + scale * u                        (scale_v non-NULL: one value per column)
+ *   h  = x' / sqrt(mean(x'^2) + eps) * w      (w NULL: not scaled)
+ *   q, q_scale = qmoe_fp8_quantize of h       (q NULL: not)
+ * y NULL: x' = x, and x_out is not written.  h and q are made of the f32 x' before
+ * it is rounded to the rows' type.  x_out may be x or y; every other output is a
+ * buffer of its own.  Replaces what follows a block in the reference: ggml_add of
+ * the residual, build_rms_norm (norm.cpp:15-26), and the norms after a block with
+ * their scale (gemma4.cpp:566 on). */
+enum qmoe_gate { QMOE_GATE_NONE = 0, QMOE_GATE_SIGMOID = 1, QMOE_GATE_SILU = 2 };
+typedef struct qmoe_norm_args {
+    const void*  x;
+    const void*  y;
+    const void*  gate;
+    const float* post_w;
+    const float* scale_v;
+    const float* w;
+    void*        x_out;
+    void*        h;
+    uint8_t*     q;
+    float*       q_scale;
+    float        scale;     /* used when scale_v is NULL */
+    float        eps;
+    int32_t      x_type;    /* of x, y, gate, x_out, h */
+    int32_t      gate_act;  /* enum qmoe_gate; QMOE_GATE_NONE iff gate is NULL */
+} qmoe_norm_args;
+int qmoe_residual_norm(const qmoe_norm_args* args, int32_t n_tokens, int32_t n_embd, void* hip_stream);
 
 /* Seeded synthetic data for tests and benchmarks, generated on the device.
  * Value i of a stream is N(mean, sigma) from a counter-based hash of

@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("QMOE_LIB") or os.path.join(PKG_DIR, "libqmoe.so")
 TYPE_F32 = 0
 TYPE_Q4_0 = 2
 TYPE_Q8_0 = 8
+TYPE_BF16 = 30
 
 QMOE_OK = 0
 QMOE_ERR_NULL = 1
@@ -73,6 +74,13 @@ EXPORTED = (
     "qmoe_residency_resident_set",
     "qmoe_residency_frequencies",
     "qmoe_residency_reset",
+    "qmoe_fp8_quantize",
+    "qmoe_fp8_matmul",
+    "qmoe_sort_tokens",
+    "qmoe_gather_tokens",
+    "qmoe_combine_tokens",
+    "qmoe_combine_tokens_backward",
+    "qmoe_residual_norm",
 )
 
 
@@ -119,6 +127,25 @@ class QmoeGgufTensor(ctypes.Structure):
         ("ne", ctypes.c_int64 * 4),
         ("file_offset", ctypes.c_uint64),
         ("nbytes", ctypes.c_uint64),
+    ]
+
+
+class QmoeNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("post_w", ctypes.c_void_p),
+        ("scale_v", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("x_out", ctypes.c_void_p),
+        ("h", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("q_scale", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("x_type", ctypes.c_int32),
+        ("gate_act", ctypes.c_int32),
     ]
 
 
@@ -241,6 +268,18 @@ def lib() -> ctypes.CDLL:
     L.qmoe_residency_frequencies.argtypes = [vp, P(ctypes.c_uint64), ctypes.c_int32]
     L.qmoe_residency_reset.restype = None
     L.qmoe_residency_reset.argtypes = [vp]
+    i32 = ctypes.c_int32
+    for name, args in (
+        ("qmoe_fp8_quantize", [vp, i32, i32, i32, i32, vp, vp, vp]),
+        ("qmoe_fp8_matmul", [vp, vp, i32, vp, vp, i32, i32, i32, vp, vp, i32, vp, i32, vp]),
+        ("qmoe_sort_tokens", [vp, i32, i32, i32, vp, vp, vp, vp, vp]),
+        ("qmoe_gather_tokens", [vp, i32, i32, i32, i32, i32, vp, vp, vp, vp]),
+        ("qmoe_combine_tokens", [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp]),
+        ("qmoe_combine_tokens_backward", [vp, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
+        ("qmoe_residual_norm", [P(QmoeNormArgs), i32, i32, vp]),
+    ):
+        getattr(L, name).restype = ctypes.c_int
+        getattr(L, name).argtypes = args
     _lib = L
     return L
 

@@ -23,6 +23,10 @@ SOURCES = [
     "expert_f16_kernels.hip",
     "expert_i8_kernels.hip",
     "misc_kernels.hip",
+    "fp8_kernels.hip",
+    "token_kernels.hip",
+    "norm_kernels.hip",
+    "ops_api.cpp",
     "qmoe_api.cpp",
     "gguf.cpp",
     "residency.cpp",

@@ -40,6 +40,42 @@ __device__ __forceinline__ uint32_t f32_to_fp16(float f) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
+// bf16 <-> fp32 (round to nearest even; NaN stays NaN)
+__device__ __forceinline__ float bf16_to_f32(uint32_t h) { return __builtin_bit_cast(float, h << 16); }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f32_pack_bf16(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+}
+
+// ---------------------------------------------------------------------------
+// e4m3 blocks of 128 values, 8 per lane of 16 lanes.
+// ---------------------------------------------------------------------------
+// The block's largest |v| (at least kFp8Tiny) in all 16 lanes, and f32(448 / it).  The
+// bits of |v| order as integers, a NaN above infinity: it wins.
+__device__ __forceinline__ float fp8_block_max(const float (&v)[8], float& inv) {
+    uint32_t m = __builtin_bit_cast(uint32_t, kFp8Tiny);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
+        m = b > m ? b : m;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        const uint32_t b = (uint32_t)__shfl_xor((int)m, o, 64);
+        m = b > m ? b : m;
+    }
+    const float top = __builtin_bit_cast(float, m);
+    inv = kFp8Max / top;
+    return top;
+}
+__device__ __forceinline__ void fp8_pack8(const float (&v)[8], float inv, uint32_t (&o)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * inv, v[4 * h + 1] * inv, 0, false);
+        o[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * inv, v[4 * h + 3] * inv, r, true);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Deterministic f64 elementary functions
 // ---------------------------------------------------------------------------

@@ -36,6 +36,44 @@ constexpr int kFixStride = 36;  // floats per listed h block: 32 values, amax's 
 constexpr int kActSilu = 0;
 constexpr int kActGeluTanh = 1;
 
+// e4m3 operands: columns per scale (rows too, for weights), the largest e4m3 value, and
+// the smallest block maximum that sets a scale.
+constexpr int kFp8Block = 128;
+constexpr float kFp8Max = 448.0f;
+constexpr float kFp8Tiny = 1e-30f;
+constexpr int kFp8ActNone = 0;
+constexpr int kFp8ActSwiglu = 1;
+constexpr int kFp8ActGeglu = 2;
+constexpr int kGateNone = 0;
+constexpr int kGateSigmoid = 1;
+constexpr int kGateSilu = 2;
+
+// y[R][N] = rows of a (e4m3 [a_rows][K], scales [a_rows][KB]) times w (e4m3 [E][N][K],
+// scales [E][NB][KB]).  offsets null: one matrix; else row r belongs to the expert with
+// offsets[e] <= r < offsets[e + 1].  rows null: row r of a, else row rows[r].
+struct Fp8Product {
+    const uint8_t* a;
+    const float* sa;
+    const uint8_t* w;
+    const float* sw;
+    const int32_t* offsets;
+    const int32_t* rows;
+    void* y;
+    int a_rows, E, N, K, R;
+    int KB, NB;     // blocks of 128 along K and N (set by the launcher)
+    bool vec_out;   // y's rows take aligned stores of four (set by the launcher)
+};
+
+struct ResidualNorm {
+    const void *x, *y, *gate;
+    const float *post_w, *scale_v, *w;
+    void *x_out, *h;
+    uint8_t* q;
+    float* q_scale;
+    float scale, eps;
+    int H, gate_act;
+};
+
 struct LayerDesc {
     int H = 0, E = 0, K = 0, F = 0, S = 0;  // n_embd, n_experts, top_k, ffn_dim, shared (0/1)
     int gu_type = 0, dn_type = 0;           // gate/up type, down type (Q4_0 or Q8_0)
@@ -233,6 +271,22 @@ hipError_t launch_unpad_rows(const float* src, int T, int hs, int hd, const floa
 // router_in = ((x*scale)*s)*w_rs with scale = 1/sqrtf(mean(x^2) + eps).
 hipError_t launch_gemma4_inputs(const float* x, const float* w_pre, const float* w_rs, int T, int H, float eps, float s,
                                 float* expert_in, float* router_in, hipStream_t stream);
+// e4m3 rows in blocks of 128 columns, after the activation of (gate, up) halves if any.
+hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols, int act, uint8_t* q, float* scale,
+                               hipStream_t stream);
+hipError_t launch_fp8_matmul(Fp8Product p, bool bf16_out, hipStream_t stream);
+// Lists of a routing, rows in their order, the weighted sum back and its gradients.
+// total: the number of assignments with a place (offsets + n_experts).
+hipError_t launch_sort_tokens(const int32_t* ids, int n_tokens, int top_k, int E, int32_t* offsets, int32_t* rows,
+                              int32_t* tokens, int32_t* place, hipStream_t stream);
+hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_cols, int top_k, const int32_t* total,
+                                const int32_t* place, void* y, hipStream_t stream);
+hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H, int top_k, const int32_t* place,
+                                 const float* w, const void* residual, void* y, hipStream_t stream);
+hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, int n_tokens, int H, int top_k,
+                                     const int32_t* total, const int32_t* place, const float* w, void* dys, float* dw,
+                                     hipStream_t stream);
+hipError_t launch_residual_norm(const ResidualNorm& p, bool bf16, int n_tokens, hipStream_t stream);
 // ggml's CPU fp16 gelu table (65536 entries): host copy, and the current device's copy.
 void gelu_table_host(uint16_t* out);
 hipError_t gelu_table_device(const uint16_t** out);
