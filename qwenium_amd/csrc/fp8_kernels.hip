@@ -4,10 +4,14 @@
 #include "qmoe_device.h"
 #include "qmoe_internal.h"
 
+#include <type_traits>
+#include <cstdlib>
+
 namespace qmoe {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
@@ -151,6 +155,25 @@ __device__ __forceinline__ bool fp8_find_tile(const Fp8Product& p, int tile, int
     return false;
 }
 
+// The row and column tile of a workgroup.  Workgroups are dealt to the 8 XCDs in turn.
+// Grouped: XCD x takes every eighth row tile with all its column tiles, so that a tile's
+// rows stay in one L2.  One matrix: each XCD a contiguous run of the order "bands of 8 row
+// tiles, column by column", whose workgroups in flight share few rows and columns.
+__device__ __forceinline__ void fp8_place(const Fp8Product& p, int bm, int nt, int& tile, int& col) {
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+    if (p.offsets) {
+        tile = (j / nt) * 8 + x;
+        col = j % nt;
+        return;
+    }
+    const int mt = (p.R + bm - 1) / bm;
+    const int at = x * (int)(gridDim.x >> 3) + j;
+    const int band = at / (8 * nt), in = at - band * 8 * nt;
+    const int high = mt - 8 * band < 8 ? mt - 8 * band : 8;  // (none past the last tile)
+    tile = high > 0 && in / high < nt ? 8 * band + in % high : mt;
+    col = high > 0 ? in / high : 0;
+}
+
 // The activation row behind product row r (-1: none, its products are zeros).
 __device__ __forceinline__ int fp8_source_row(const Fp8Product& p, int r) {
     if (!p.rows) return r;
@@ -158,17 +181,30 @@ __device__ __forceinline__ int fp8_source_row(const Fp8Product& p, int r) {
     return s >= 0 && s < p.a_rows ? s : -1;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void fp8_store4(const Fp8Product& p, int r, int n, const float (&v)[4]) {
+// C consecutive columns (4 or 8) of a row from column n on; those past N are left out.
+template <bool BF16, int C>
+__device__ __forceinline__ void fp8_store(const Fp8Product& p, int r, int n, const float (&v)[C]) {
     const uint64_t at = (uint64_t)r * p.N + n;
-    if (p.vec_out && n + 4 <= p.N) {
-        if (BF16)
-            *(uint2*)((uint16_t*)p.y + at) = make_uint2(f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]));
-        else
-            *(f32x4*)((float*)p.y + at) = f32x4{v[0], v[1], v[2], v[3]};
+    if (p.vec_out && n + C <= p.N) {
+        if constexpr (BF16) {
+            uint32_t o[C / 2];
+#pragma unroll
+            for (int i = 0; i < C / 2; ++i) o[i] = f32_pack_bf16(v[2 * i], v[2 * i + 1]);
+            if constexpr (C == 4) {
+                *(uint2*)((uint16_t*)p.y + at) = make_uint2(o[0], o[1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < C / 8; ++i)
+                    *(u32x4*)((uint16_t*)p.y + at + 8 * i) = u32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < C / 4; ++i)
+                *(f32x4*)((float*)p.y + at + 4 * i) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < C; ++i)
             if (n + i < p.N) {
                 if (BF16) ((uint16_t*)p.y)[at + i] = (uint16_t)f32_pack_bf16(v[i], 0.0f);
                 else ((float*)p.y)[at + i] = v[i];
@@ -267,7 +303,244 @@ __global__ __launch_bounds__(256) void k_fp8_stream(Fp8Product p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             v[c] = (s_part[0][m][q + c] + s_part[1][m][q + c]) + (s_part[2][m][q + c] + s_part[3][m][q + c]);
-        if (row0 + m < end && n0 + q < p.N) fp8_store4<BF16>(p, row0 + m, n0 + q, v);
+        if (row0 + m < end && n0 + q < p.N) fp8_store<BF16, 4>(p, row0 + m, n0 + q, v);
+    }
+}
+
+// Many rows: a workgroup of WM x WN waves makes a tile of 16 MS WM rows and 16 NS WN
+// columns.  Each step of 128 columns of K comes straight to LDS (two buffers, one
+// step ahead): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
+// (row & 7), so that the 16 rows of a fragment meet all banks.  The 16-row subtiles
+// go to the WM waves in turn and those without rows are left out (MI: how many).
+// A wave-uniform read-only value through the scalar cache: no vector memory load, whose
+// wait would be one for all direct loads before it.
+__device__ __forceinline__ float scalar_load(const float* p) {
+    return *(const __attribute__((address_space(4))) float*)(uintptr_t)p;
+}
+// s_waitcnt's operand for at most n vector memory operations in flight
+constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
+// A workgroup barrier after this wave's own LDS accesses; direct loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+template <int WM, int WN, int MS, int NS, int ST, bool BF16>
+struct Fp8Tile {
+    static constexpr int kWaves = WM * WN, kBM = 16 * MS * WM, kBN = 16 * NS * WN;
+    static constexpr int kScaleLoads = (kBM + 63) / 64;
+    static constexpr int kStage = (kBM + kBN) * kFp8Block;  // rows, weights
+    static constexpr int kScales = 1024 * kScaleLoads;      // row scales of four steps: two buffers behind the stages
+    static constexpr int kLds = ST * kStage + 2 * kScales + 64 * kScaleLoads;
+    // Columns that a lane stores together: 16 bytes.  Of 4 kCols columns, 4 a + c of P = kCols / 4 subtiles each,
+    // weight row 4 P a + 4 n + c is the MFMA's row 4 a + c of subtile n, so that lane group a holds 4 P consecutive
+    // columns and a wave's four groups 64 bytes of a row.  The row's pieces lie at slots piece ^ slot_w(row): the
+    // eight rows that a quarter of a wave reads (a = 0, 1 or 2, 3; c = 0..3) have eight slots.
+    static constexpr int P = BF16 && NS > 1 ? 2 : 1, kCols = 4 * P;
+    static_assert(NS % P == 0, "whole groups of subtiles");
+    static __host__ __device__ constexpr int slot_w(int row) { return (row & 3) | (row / kCols & 1) << 2; }
+    static constexpr int kGroupsA = (kBM / 8 + kWaves - 1) / kWaves;
+    static constexpr int kLoads = kGroupsA + kBN / 8 / kWaves;  // of one wave, a step, without scales
+    static_assert(kBM % 32 == 0 && kBN % (8 * kWaves) == 0, "whole loads per wave");
+    static_assert(16 * NS <= kFp8Block, "a wave's columns share one scale");
+};
+
+template <int WM, int WN, int MS, int NS, int ST, bool BF16>
+__global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
+    using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
+    extern __shared__ uint8_t s_dyn[];
+    const int nt = (p.N + T::kBN - 1) / T::kBN;
+    int tile, n0, e, row0, end;
+    fp8_place(p, T::kBM, nt, tile, n0);
+    n0 *= T::kBN;
+    if (!fp8_find_tile(p, T::kBM, tile, e, row0, end)) return;
+    const int nrows = end - row0 < T::kBM ? end - row0 : T::kBM;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wm = wave % WM, wn = wave / WM;
+    const int KB = p.KB;
+
+    // this lane's share of the loads: groups of 8 rows, 8 lanes a row
+    constexpr int kGA = T::kGroupsA, kGW = T::kBN / 8 / T::kWaves;
+    const int piece = 16 * ((lane & 7) ^ (lane >> 3));
+    const int piece_w = 16 * ((lane & 7) ^ T::slot_w(8 * wave + (lane >> 3)));
+    static_assert(T::slot_w(8 * T::kWaves) == 0, "the same slots in every group of a wave");
+    // (a tile whose row groups do not divide among the waves: the last ones load some again)
+    auto group_a = [&](int i) {
+        const int g = wave + T::kWaves * i;
+        return T::kBM / 8 % T::kWaves == 0 || g < T::kBM / 8 ? g : g - T::kWaves;
+    };
+    const uint8_t* ga[kGA];
+#pragma unroll
+    for (int i = 0; i < kGA; ++i) {
+        const int r = 8 * group_a(i) + (lane >> 3);
+        const int s = fp8_source_row(p, row0 + (r < nrows ? r : nrows - 1));
+        ga[i] = p.a + (uint64_t)(s < 0 ? 0 : s) * p.K;
+    }
+    const uint8_t* const wt = p.w + ((uint64_t)e * p.N + n0) * p.K;  // the tile's weights, offsets below 2^32
+    uint32_t gw[kGW];
+#pragma unroll
+    for (int i = 0; i < kGW; ++i) {
+        const int n = 8 * (wave + T::kWaves * i) + (lane >> 3);
+        gw[i] = (uint32_t)(n < p.N - n0 ? n : p.N - n0 - 1) * (uint32_t)p.K;
+    }
+    const float* gs = nullptr;
+    uint8_t* s_none = s_dyn + ST * T::kStage + 2 * T::kScales;  // rows without a source (read after the loop's barriers)
+    if (wave < T::kScaleLoads) {
+        const int r = 64 * wave + lane;
+        const int s = fp8_source_row(p, row0 + (r < nrows ? r : nrows - 1));
+        gs = p.sa + (uint64_t)(s < 0 ? 0 : s) * KB;
+        s_none[r] = s < 0;
+    }
+    // load l of step b into buffer buf: the rows' groups, the weights', the row scales
+    const uint32_t lds0 = lds_addr(s_dyn);
+    auto load = [&](int l, int b, int buf) {
+        const int c = b * kFp8Block + (l < kGA ? piece : piece_w);
+        const int at = c < p.K ? c : p.K - 16;  // past K: any valid piece, its weights are zeroed below
+        const uint32_t base = lds0 + buf * T::kStage;
+        if (l < kGA) dma_lds16_at(ga[l] + at, base + 1024 * group_a(l));
+        else dma_lds16(wt, gw[l - kGA] + (uint32_t)at, base + T::kBM * kFp8Block + 1024 * (wave + T::kWaves * (l - kGA)));
+    };
+    // The row scales of steps b .. b + 3, by the waves 0 .. kScaleLoads - 1: 64 rows each, 16 bytes a row
+    // (a row's scales lie KB apart: one 64-row load of single scales costs as much).  Where KB is no
+    // multiple of 4, four loads of one step each.
+    const bool quads = KB % 4 == 0 && ((uintptr_t)p.sa & 15) == 0;
+    auto load_scales = [&](int b) {
+        if (wave >= T::kScaleLoads) return;
+        const uint32_t base = lds0 + ST * T::kStage + (b >> 2 & 1) * T::kScales + 1024 * wave;
+        if (quads) {
+            dma_lds16_at(gs + b, base);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dma_lds4_at(gs + (b + i < KB ? b + i : KB - 1), base + 256 * i);
+        }
+    };
+    const int scale_row = quads ? 16 : 4, scale_step = quads ? 4 : 256;  // LDS distances
+
+    const int nw0 = n0 + 16 * NS * wn;  // this wave's columns
+    const float* sw = p.sw + ((uint64_t)e * p.NB + (nw0 < p.N ? nw0 >> 7 : 0)) * KB;
+    const int fr = lane & 15, fg = lane >> 4;
+    const int piece0 = fr * kFp8Block + 16 * (fg ^ (fr & 7)), piece1 = piece0 ^ 64;  // (fg + 4) ^ .. = (fg ^ ..) ^ 4
+    const int fw = T::kCols * (fr >> 2) + (fr & 3);  // this lane's weight row of subtile 0
+    const int wpiece0 = fw * kFp8Block + 16 * (fg ^ T::slot_w(fw)), wpiece1 = wpiece0 ^ 64;
+    f32x4 acc[MS][NS] = {};
+    auto run = [&](auto mi_c) {
+        constexpr int MI = decltype(mi_c)::value;
+        int buf = 0, next = ST - 1;
+        float ws_next = scalar_load(sw);
+        // TAIL: step b is the last and shorter than a block
+        auto step = [&](int b, auto tail_c) {
+            constexpr bool TAIL = decltype(tail_c)::value;
+            // step b has landed (at most the ST - 2 after it are in flight) ...
+            // (a wave's scale loads come before its stage's: they have landed with it)
+            if (!TAIL && b + ST - 2 < KB) __builtin_amdgcn_s_waitcnt(vm_wait((ST - 2) * T::kLoads));
+            else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+            lds_barrier();  // ... for every wave, and the oldest buffer is no longer read
+            const float ws = ws_next;
+            ws_next = scalar_load(sw + (b + 1 < KB ? b + 1 : b));
+            const uint8_t* st = s_dyn + buf * T::kStage;
+            const uint8_t* scales = s_dyn + ST * T::kStage + (b >> 2 & 1) * T::kScales + (b & 3) * scale_step + fr * scale_row;
+            i32x4 al[2], ah[2], wl[NS], wh[NS];
+            float rs[2];
+            auto rows = [&](int i) {
+                const int sub = WM * i + wm;
+                al[i & 1] = *(const i32x4*)(st + 16 * sub * kFp8Block + piece0);
+                ah[i & 1] = *(const i32x4*)(st + 16 * sub * kFp8Block + piece1);
+                // (subtile sub is rows 16 (sub % 4) .. of load sub / 4)
+                rs[i & 1] = *(const float*)(scales + 1024 * (sub >> 2) + 16 * (sub & 3) * scale_row);
+            };
+            rows(0);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                const uint8_t* w = st + (T::kBM + 16 * NS * wn + 4 * T::kCols * (n / T::P) + 4 * (n % T::P)) * kFp8Block;
+                wl[n] = *(const i32x4*)(w + wpiece0);
+                wh[n] = *(const i32x4*)(w + wpiece1);
+                if (TAIL) {
+                    if (16 * fg >= p.K - b * kFp8Block) wl[n] = i32x4{};
+                    if (16 * (fg + 4) >= p.K - b * kFp8Block) wh[n] = i32x4{};
+                }
+            }
+            f16x8 wf[BF16 ? 1 : NS][4];
+            if constexpr (!BF16) {
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    wf[n][0] = fp8_to_f16(wl[n][0], wl[n][1]);
+                    wf[n][1] = fp8_to_f16(wl[n][2], wl[n][3]);
+                    wf[n][2] = fp8_to_f16(wh[n][0], wh[n][1]);
+                    wf[n][3] = fp8_to_f16(wh[n][2], wh[n][3]);
+                }
+            }
+            const bool more = !TAIL && b + ST - 1 < KB;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                if (i + 1 < MI) rows(i + 1);
+                const float s = ws * rs[i & 1];
+                if constexpr (BF16) {
+                    const i32x8 af = __builtin_shufflevector(al[i & 1], ah[i & 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    f32x4 t[NS];
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+                        t[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                            __builtin_shufflevector(wl[n], wh[n], 0, 1, 2, 3, 4, 5, 6, 7), af, f32x4{}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                    for (int n = 0; n < NS; ++n)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(s, t[n][c], acc[i][n][c]);
+                } else {
+                    const f16x8 a0 = fp8_to_f16(al[i & 1][0], al[i & 1][1]), a1 = fp8_to_f16(al[i & 1][2], al[i & 1][3]);
+                    const f16x8 a2 = fp8_to_f16(ah[i & 1][0], ah[i & 1][1]), a3 = fp8_to_f16(ah[i & 1][2], ah[i & 1][3]);
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) {
+                        f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][0], a0, f32x4{}, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][1], a1, t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][2], a2, t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][3], a3, t, 0, 0, 0);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(s, t[c], acc[i][n][c]);
+                    }
+                }
+                // a later step's loads: with two buffers at once, so that they have this step to
+                // land; with more, a few after each subtile
+                if (!TAIL && more) {
+                    if (i == 0 && (b + ST - 1) % 4 == 0) load_scales(b + ST - 1);
+#pragma unroll
+                    for (int l = 0; l < T::kLoads; ++l)
+                        if (ST == 2 ? i == 0 : l >= i * T::kLoads / MI && l < (i + 1) * T::kLoads / MI) load(l, b + ST - 1, next);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            buf = buf + 1 == ST ? 0 : buf + 1;
+            next = next + 1 == ST ? 0 : next + 1;
+        };
+        const int whole = p.K / kFp8Block;
+        for (int b = 0; b < whole; ++b) step(b, std::false_type{});
+        if (whole < KB) step(whole, std::true_type{});
+    };
+    load_scales(0);
+#pragma unroll
+    for (int b = 0; b < ST - 1; ++b)
+        if (b < KB)
+#pragma unroll
+            for (int l = 0; l < T::kLoads; ++l) load(l, b, b);
+    const int subs = (nrows + 15) >> 4;                     // subtiles with rows
+    const int mine = subs > wm ? (subs - wm + WM - 1) / WM : 0;  // ... of this wave
+    if (mine > MS / 2) run(std::integral_constant<int, MS>{});
+    else if (mine > MS / 4) run(std::integral_constant<int, MS / 2>{});
+    else run(std::integral_constant<int, MS / 4>{});
+
+#pragma unroll
+    for (int i = 0; i < MS; ++i) {
+        const int m = 16 * (WM * i + wm) + fr;
+        if (m >= nrows) continue;
+        const bool none = s_none[m];
+#pragma unroll
+        for (int n = 0; n < NS; n += T::P) {
+            const int col = nw0 + 16 * n + T::kCols * fg;
+            float v[T::kCols];
+#pragma unroll
+            for (int c = 0; c < T::kCols; ++c) v[c] = none ? 0.0f : acc[i][n + (c >> 2)][c & 3];
+            if (col < p.N) fp8_store<BF16, T::kCols>(p, row0 + m, col, v);
+        }
     }
 }
 
@@ -287,12 +560,40 @@ static hipError_t launch_stream(const Fp8Product& p, bool bf16, hipStream_t stre
     return hipGetLastError();
 }
 
+template <int WM, int WN, int MS, int NS, int ST, bool BF16>
+static hipError_t launch_tile(const Fp8Product& p, hipStream_t stream) {
+    using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
+    const int64_t tiles = fp8_max_tiles(p, T::kBM), nt = (p.N + T::kBN - 1) / T::kBN;
+    const int64_t blocks = p.offsets ? (tiles + 7) / 8 * 8 * nt : (tiles * nt + 7) / 8 * 8;
+    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_fp8_tile<WM, WN, MS, NS, ST, BF16>), dim3((unsigned)blocks), dim3(64 * T::kWaves), T::kLds, stream, p);
+    return hipGetLastError();
+}
+
 hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     if (p.R <= 0) return hipSuccess;
     p.KB = (p.K + kFp8Block - 1) / kFp8Block;
     p.NB = (p.N + kFp8Block - 1) / kFp8Block;
-    p.vec_out = p.N % 4 == 0 && ((uintptr_t)p.y & 15u) == 0;
+    p.vec_out = p.N % 8 == 0 && ((uintptr_t)p.y & 15u) == 0;
     const int64_t mean = p.offsets ? p.R / p.E : p.R;  // rows per weight matrix
+    if (const char* v = getenv("QMOE_X")) {
+        const int x = atoi(v);
+        if (x == 1) return bf16 ? launch_tile<2, 4, 8, 4, 2, true>(p, stream) : launch_tile<2, 4, 8, 4, 2, false>(p, stream);
+        if (x == 2) return bf16 ? launch_tile<2, 2, 4, 4, 2, true>(p, stream) : launch_tile<2, 2, 4, 4, 2, false>(p, stream);
+        if (x == 12) return bf16 ? launch_tile<1, 4, 4, 2, 3, true>(p, stream) : launch_tile<1, 4, 4, 2, 3, false>(p, stream);
+        if (x == 18) return bf16 ? launch_tile<2, 4, 4, 4, 3, true>(p, stream) : launch_tile<2, 4, 4, 4, 3, false>(p, stream);
+        if (x == 19) return bf16 ? launch_tile<1, 4, 4, 1, 3, true>(p, stream) : launch_tile<1, 4, 4, 1, 3, false>(p, stream);
+        if (x == 22) return bf16 ? launch_tile<2, 4, 5, 2, 2, true>(p, stream) : launch_tile<2, 4, 5, 2, 2, false>(p, stream);
+        if (x == 23) return bf16 ? launch_tile<2, 4, 5, 4, 2, true>(p, stream) : launch_tile<2, 4, 5, 4, 2, false>(p, stream);
+        if (x == 24) return bf16 ? launch_tile<2, 4, 5, 2, 3, true>(p, stream) : launch_tile<2, 4, 5, 2, 3, false>(p, stream);
+        if (x == 25) return bf16 ? launch_tile<2, 4, 6, 2, 2, true>(p, stream) : launch_tile<2, 4, 6, 2, 2, false>(p, stream);
+        if (x == 26) return bf16 ? launch_tile<2, 4, 6, 4, 2, true>(p, stream) : launch_tile<2, 4, 6, 4, 2, false>(p, stream);
+        if (x == 27) return bf16 ? launch_tile<2, 2, 5, 4, 2, true>(p, stream) : launch_tile<2, 2, 5, 4, 2, false>(p, stream);
+        if (x == 28) return bf16 ? launch_tile<1, 4, 10, 2, 2, true>(p, stream) : launch_tile<1, 4, 10, 2, 2, false>(p, stream);
+        if (x == 8) return launch_stream<4, 1>(p, bf16, stream);
+        if (x == 9) return launch_stream<2, 2>(p, bf16, stream);
+        if (x == 10) return launch_stream<1, 4>(p, bf16, stream);
+    }
     if (mean >= 32) return launch_stream<4, 1>(p, bf16, stream);
     if (mean >= 12) return launch_stream<2, 2>(p, bf16, stream);
     return launch_stream<1, 4>(p, bf16, stream);
