@@ -5,7 +5,6 @@
 #include "qmoe_internal.h"
 
 #include <type_traits>
-#include <cstdlib>
 
 namespace qmoe {
 
@@ -221,7 +220,7 @@ __device__ __forceinline__ f16x8 fp8_to_f16(int a, int b) {
     return f16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
 }
 
-// Few rows: a workgroup makes 16 columns of 16 MT rows.  Its four waves take the
+// Few rows (MT 1 or 2): a workgroup makes 16 columns of 16 MT rows.  Its four waves take the
 // k blocks in turn, straight from memory into the MFMA operands, U blocks in flight;
 // their sums are joined in LDS in wave order.
 template <int MT, int U, bool BF16>
@@ -342,7 +341,7 @@ struct Fp8Tile {
     static __host__ __device__ constexpr int slot_w(int row) { return (row & 3) | (row / kCols & 1) << 2; }
     static constexpr int kGroupsA = (kBM / 8 + kWaves - 1) / kWaves;
     static constexpr int kLoads = kGroupsA + kBN / 8 / kWaves;  // of one wave, a step, without scales
-    static_assert(kBM % 32 == 0 && kBN % (8 * kWaves) == 0, "whole loads per wave");
+    static_assert(kBM % 16 == 0 && kBN % (8 * kWaves) == 0, "whole loads per wave");
     static_assert(16 * NS <= kFp8Block, "a wave's columns share one scale");
 };
 
@@ -544,6 +543,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     }
 }
 
+constexpr int64_t kFp8Cus = 256;  // CUs of the MI355X
+
 // Tiles that the rows of a product fill at most, whatever their split over experts.
 static int64_t fp8_max_tiles(const Fp8Product& p, int tile) {
     if (!p.offsets) return (p.R + tile - 1) / tile;
@@ -561,7 +562,7 @@ static hipError_t launch_stream(const Fp8Product& p, bool bf16, hipStream_t stre
 }
 
 template <int WM, int WN, int MS, int NS, int ST, bool BF16>
-static hipError_t launch_tile(const Fp8Product& p, hipStream_t stream) {
+static hipError_t launch_tile_as(const Fp8Product& p, hipStream_t stream) {
     using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
     const int64_t tiles = fp8_max_tiles(p, T::kBM), nt = (p.N + T::kBN - 1) / T::kBN;
     const int64_t blocks = p.offsets ? (tiles + 7) / 8 * 8 * nt : (tiles * nt + 7) / 8 * 8;
@@ -569,34 +570,45 @@ static hipError_t launch_tile(const Fp8Product& p, hipStream_t stream) {
     hipLaunchKernelGGL((k_fp8_tile<WM, WN, MS, NS, ST, BF16>), dim3((unsigned)blocks), dim3(64 * T::kWaves), T::kLds, stream, p);
     return hipGetLastError();
 }
+template <int WM, int WN, int MS, int NS, int ST>
+static hipError_t launch_tile(const Fp8Product& p, bool bf16, hipStream_t stream) {
+    return bf16 ? launch_tile_as<WM, WN, MS, NS, ST, true>(p, stream) : launch_tile_as<WM, WN, MS, NS, ST, false>(p, stream);
+}
 
 hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     if (p.R <= 0) return hipSuccess;
     p.KB = (p.K + kFp8Block - 1) / kFp8Block;
     p.NB = (p.N + kFp8Block - 1) / kFp8Block;
     p.vec_out = p.N % 8 == 0 && ((uintptr_t)p.y & 15u) == 0;
-    const int64_t mean = p.offsets ? p.R / p.E : p.R;  // rows per weight matrix
-    if (const char* v = getenv("QMOE_X")) {
-        const int x = atoi(v);
-        if (x == 1) return bf16 ? launch_tile<2, 4, 8, 4, 2, true>(p, stream) : launch_tile<2, 4, 8, 4, 2, false>(p, stream);
-        if (x == 2) return bf16 ? launch_tile<2, 2, 4, 4, 2, true>(p, stream) : launch_tile<2, 2, 4, 4, 2, false>(p, stream);
-        if (x == 12) return bf16 ? launch_tile<1, 4, 4, 2, 3, true>(p, stream) : launch_tile<1, 4, 4, 2, 3, false>(p, stream);
-        if (x == 18) return bf16 ? launch_tile<2, 4, 4, 4, 3, true>(p, stream) : launch_tile<2, 4, 4, 4, 3, false>(p, stream);
-        if (x == 19) return bf16 ? launch_tile<1, 4, 4, 1, 3, true>(p, stream) : launch_tile<1, 4, 4, 1, 3, false>(p, stream);
-        if (x == 22) return bf16 ? launch_tile<2, 4, 5, 2, 2, true>(p, stream) : launch_tile<2, 4, 5, 2, 2, false>(p, stream);
-        if (x == 23) return bf16 ? launch_tile<2, 4, 5, 4, 2, true>(p, stream) : launch_tile<2, 4, 5, 4, 2, false>(p, stream);
-        if (x == 24) return bf16 ? launch_tile<2, 4, 5, 2, 3, true>(p, stream) : launch_tile<2, 4, 5, 2, 3, false>(p, stream);
-        if (x == 25) return bf16 ? launch_tile<2, 4, 6, 2, 2, true>(p, stream) : launch_tile<2, 4, 6, 2, 2, false>(p, stream);
-        if (x == 26) return bf16 ? launch_tile<2, 4, 6, 4, 2, true>(p, stream) : launch_tile<2, 4, 6, 4, 2, false>(p, stream);
-        if (x == 27) return bf16 ? launch_tile<2, 2, 5, 4, 2, true>(p, stream) : launch_tile<2, 2, 5, 4, 2, false>(p, stream);
-        if (x == 28) return bf16 ? launch_tile<1, 4, 10, 2, 2, true>(p, stream) : launch_tile<1, 4, 10, 2, 2, false>(p, stream);
-        if (x == 8) return launch_stream<4, 1>(p, bf16, stream);
-        if (x == 9) return launch_stream<2, 2>(p, bf16, stream);
-        if (x == 10) return launch_stream<1, 4>(p, bf16, stream);
+    // Workgroups of rows x cols tiles (grouped: at most).
+    auto wgs = [&](int rows, int cols) { return fp8_max_tiles(p, rows) * ((p.N + cols - 1) / cols); };
+    // A grid of at most two workgroups per CU that streams its operands once: latency.
+    if (wgs(p.offsets ? 16 : 32, 16) <= 2 * kFp8Cus)
+        return p.offsets || p.R <= 16 ? launch_stream<1, 4>(p, bf16, stream) : launch_stream<2, 2>(p, bf16, stream);
+    if (!p.offsets) {
+        // The largest tile that gives every CU a workgroup.  Rows x 4096 x 4096, bf16, us with tiles of
+        // 256x256 / 128x256 / 64x128 / 64x64: 4096 rows 68 / 79 / 99 / 125, 2048 59 / 40 / 51 / 65,
+        // 1024 58 / 35 / 27 / 37, 256 56 / 34 / 19 / 17.
+        if (wgs(256, 256) >= kFp8Cus) return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
+        if (wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
+    } else {
+        // By the rows an expert has on average: the tile that holds most experts' rows with few rows to
+        // spare.  256 experts of 1024 x 2048, bf16, us with 256x256 / 160x128 / 128x256 / 64x128: 32 rows
+        // 123 / 107 / 104 / 99, 64 rows 133 / 121 / 114 / 125, 128 rows 153 / 158 / 154 / 194, 187 rows
+        // 182 / 210 / 204 / 259; 128 experts of 2816 x 704: 125 rows 109 / 99 / 109 / 118; f32, 128 rows
+        // 240 / 206 / 222 / 241.
+        const int64_t mean = p.R / p.E;
+        if (mean >= 110) {
+            const int64_t most = mean + mean / 7;  // (most experts' rows, evenly drawn)
+            if ((most + 255) / 256 * 256 < (most + 159) / 160 * 160 && wgs(256, 256) >= kFp8Cus)
+                return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
+            if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
+        } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
+            return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
+        }
     }
-    if (mean >= 32) return launch_stream<4, 1>(p, bf16, stream);
-    if (mean >= 12) return launch_stream<2, 2>(p, bf16, stream);
-    return launch_stream<1, 4>(p, bf16, stream);
+    if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
+    return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
 }
 
 }  // namespace qmoe

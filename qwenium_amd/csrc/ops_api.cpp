@@ -87,7 +87,7 @@ int qmoe_fp8_matmul(const uint8_t* a, const float* a_scale, int32_t a_rows, cons
                     void* y, int32_t y_type, void* hip_stream) {
     qmoe::clear_error();
     QMOE_TRY(row_type("y_type", y_type));
-    QMOE_TRY(in_range("n_rows", n_rows, 0, INT32_MAX));
+    QMOE_TRY(in_range("n_rows", n_rows, 0, 1 << 30));
     QMOE_TRY(in_range("a_rows", a_rows, 0, INT32_MAX));
     QMOE_TRY(in_range("n", n, 1, 1 << 24));
     QMOE_TRY(in_range("k", k, 16, 1 << 20));
