@@ -69,21 +69,29 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+_NO_STREAM = contextlib.nullcontext()
+
+
 def _on(stream):
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+    return _NO_STREAM if stream is None else torch.cuda.stream(stream)
 
 
 def _launch(fn, device, stream, *args) -> None:
     """Calls fn(*args, stream) with the operands' device current."""
+    index = device.index
     if stream is None:
-        stream = torch.cuda.current_stream(device)
+        # torch.cuda.current_stream(device).cuda_stream without the Stream object around
+        # it (1.9 us of a 5 us call)
+        handle = torch._C._cuda_getCurrentRawStream(index)
     elif stream.device != device:
         raise ValueError(f"stream expected one of {device}, got one of {stream.device}")
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream.cuda_stream)
+    else:
+        handle = stream.cuda_stream
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, handle)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream.cuda_stream)
+            rc = fn(*args, handle)
     if rc:
         check(rc)
 
@@ -156,21 +164,37 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     return out
 
 
-@dataclasses.dataclass
 class TokenOrder:
     """The lists of a routing topk_idx [T, k] (assignment a = t * k + j), int32:
     offsets [E+1] each expert's first row and the number of rows; rows [T*k] the
     assignments grouped by expert, ascending within one; tokens [T*k] their tokens;
     place [T, k] each assignment's index in rows.  Dropped assignments (ids outside
-    [0, E)) have place -1; rows and tokens are -1 from offsets[E] on."""
-    offsets: torch.Tensor
-    rows: torch.Tensor
-    tokens: torch.Tensor
-    place: torch.Tensor
+    [0, E)) have place -1; rows and tokens are -1 from offsets[E] on.  Read-only:
+    the tensors are checked once, here."""
+    __slots__ = ("_offsets", "_rows", "_tokens", "_place", "_dims")
 
-    @property
-    def n_experts(self) -> int:
-        return self.offsets.shape[0] - 1
+    def __init__(self, offsets: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, place: torch.Tensor):
+        if not isinstance(place, torch.Tensor) or place.dim() != 2:
+            raise _want("place", "an int32 [T, k] tensor", place)
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 2:
+            raise _want("offsets", "an int32 [n_experts + 1] tensor", offsets)
+        T, k = place.shape
+        _kept("place", place, place.device, (T, k), torch.int32)
+        _kept("offsets", offsets, place.device, tuple(offsets.shape), torch.int32)
+        _kept("rows", rows, place.device, (T * k,), torch.int32)
+        _kept("tokens", tokens, place.device, (T * k,), torch.int32)
+        self._set(offsets, rows, tokens, place)
+
+    def _set(self, offsets, rows, tokens, place):
+        self._offsets, self._rows, self._tokens, self._place = offsets, rows, tokens, place
+        self._dims = (*place.shape, offsets.shape[0] - 1)
+        return self
+
+    offsets = property(lambda self: self._offsets)
+    rows = property(lambda self: self._rows)
+    tokens = property(lambda self: self._tokens)
+    place = property(lambda self: self._place)
+    n_experts = property(lambda self: self._dims[2])
 
 
 def sort_tokens(topk_idx: torch.Tensor, n_experts: int, *, stream=None) -> TokenOrder:
@@ -181,25 +205,20 @@ def sort_tokens(topk_idx: torch.Tensor, n_experts: int, *, stream=None) -> Token
         n_experts = int(n_experts)
         if n_experts < 1:
             raise ValueError(f"n_experts expected at least 1, got {n_experts}")
-        A, head = T * k, (n_experts + 4) // 4 * 4
-        # one buffer: the lists' ends padded to 16 bytes
-        pad = (A + 3) // 4 * 4
-        buf = torch.empty(head + 3 * pad, dtype=torch.int32, device=idx.device)
-        offsets, rows, tokens, place = (buf[:n_experts + 1], buf[head:head + A], buf[head + pad:head + pad + A],
-                                        buf[head + 2 * pad:head + 2 * pad + A].view(T, k))
+        A = T * k
+        place, rows, tokens, offsets = torch.empty(3 * A + n_experts + 1, dtype=torch.int32, device=idx.device).split(
+            (A, A, A, n_experts + 1))  # one allocation
+        place = place.view(T, k)
         _launch(lib().qmoe_sort_tokens, idx.device, stream, idx.data_ptr(), T, k, n_experts, offsets.data_ptr(),
                 rows.data_ptr(), tokens.data_ptr(), place.data_ptr())
-    return TokenOrder(offsets, rows, tokens, place)
+    return object.__new__(TokenOrder)._set(offsets, rows, tokens, place)
 
 
 def _order(order: TokenOrder, device) -> tuple:
     """(T, k, E) of an order on `device`."""
-    place, offsets = order.place, order.offsets
-    if place.dim() != 2:
-        raise _want("order.place", "an int32 [T, k] tensor", place)
-    _kept("order.place", place, device, tuple(place.shape), torch.int32)
-    _kept("order.offsets", offsets, device, tuple(offsets.shape), torch.int32)
-    return place.shape[0], place.shape[1], offsets.shape[0] - 1
+    if not isinstance(order, TokenOrder) or order._place.device != device:
+        raise _want("order", f"a TokenOrder on {device}", order._place if isinstance(order, TokenOrder) else order)
+    return order._dims
 
 
 def gather_tokens(x: torch.Tensor, order: TokenOrder, *, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
