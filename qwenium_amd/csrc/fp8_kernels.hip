@@ -12,7 +12,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------------------
 // Quantization.  Block b of a row: m = max(|v|, kFp8Tiny) over its 128 columns
@@ -30,24 +29,6 @@ __device__ __forceinline__ float fp8_act(int act, float g, float u) {
     return g / (1.0f + expf(-z)) * u;
 }
 
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load8(const void* x, uint64_t at, int n, float (&v)[8]) {
-    if constexpr (VEC && BF16) {
-        const u16x8 r = *(const u16x8*)((const uint16_t*)x + at);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(r[i]);
-    } else if constexpr (VEC) {
-        const f32x4 r = *(const f32x4*)((const float*)x + at), s = *(const f32x4*)((const float*)x + at + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = r[i], v[4 + i] = s[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = i >= n ? 0.0f : BF16 ? bf16_to_f32(((const uint16_t*)x)[at + i]) : ((const float*)x)[at + i];
-    }
-}
-
-// VEC: the columns are a multiple of 8 and every row starts 16-byte aligned
 template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_blocks, int cols, int act, uint8_t* q,
                                                       float* scale) {

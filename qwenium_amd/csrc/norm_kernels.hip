@@ -11,89 +11,130 @@ namespace qmoe {
 //   x' = x + scale * u                             (scale: one value or one per column)
 //   h  = x' / sqrt(mean(x'^2) + eps) * w           (the next block's norm)
 //   (q, q_scale) = h in e4m3, blocks of 128        (q)
-// One workgroup per row; the row's x' stays in LDS as f32 between its two
-// passes.  The sums of squares are f64 of the f32 squares.  h and q come from the
-// f32 x', not from its rounding to the rows' type.
+// One workgroup per row, 8 columns a thread (a second 8 above 8192 columns), so
+// that the row stays in registers between the loads and the stores: each operand
+// is read once, and 16 neighbouring threads hold a block of 128 columns.  The sums
+// of squares are f64 of the f32 squares (a thread's in turn, the tree over a wave's
+// lanes, the waves in turn).  h and q come from the f32 x', not from its rounding
+// to the rows' type.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ double block_sum_f64(double v, double* s, int nw) {
+__device__ __forceinline__ double block_sum_f64(double v, double* s) {
     v = dpp_sum_f64<64>(v);
-    __syncthreads();  // s is free again
     if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = v;
     __syncthreads();
     double t = 0.0;
-    for (int i = 0; i < nw; ++i) t += s[i];
+    for (int i = 0; i < (int)blockDim.x >> 6; ++i) t += s[i];
     return t;
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(256) void k_residual_norm(ResidualNorm p) {
-    extern __shared__ float s_row[];
-    __shared__ double s_sum[4];
+template <bool BF16, bool VEC, int NP>
+__global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
+    __shared__ double s_sum[2][16];
     const uint64_t row = (uint64_t)blockIdx.x * p.H;
     const int H = p.H;
-    auto at = [&](const void* m, int i) {
-        return BF16 ? bf16_to_f32(((const uint16_t*)m)[row + i]) : ((const float*)m)[row + i];
-    };
-    auto put = [&](void* m, int i, float v) {
-        if (BF16) ((uint16_t*)m)[row + i] = (uint16_t)f32_pack_bf16(v, 0.0f);
-        else ((float*)m)[row + i] = v;
-    };
-    float post = 1.0f;
-    if (p.y && p.post_w) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < H; i += 256) {
-            const float v = at(p.y, i);
-            s += (double)(v * v);
+    float v[NP][8] = {}, u[NP][8] = {}, g[NP][8] = {};
+    int c0[NP], n[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        c0[i] = 8 * ((int)threadIdx.x + i * (int)blockDim.x);
+        n[i] = H - c0[i];  // columns from c0 on: none or some of the 8 may exist
+        if (n[i] <= 0) continue;
+        load8<BF16, VEC>(p.x, row + c0[i], n[i], v[i]);
+        if (p.y) load8<BF16, VEC>(p.y, row + c0[i], n[i], u[i]);
+        if (p.gate) load8<BF16, VEC>(p.gate, row + c0[i], n[i], g[i]);
+    }
+    if (p.y) {
+        float post = 1.0f;
+        if (p.post_w) {
+            double s = 0.0;
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s += (double)(u[i][c] * u[i][c]);
+            post = rms_scale_from_ssq(block_sum_f64(s, s_sum[0]), H, p.eps);
         }
-        post = rms_scale_from_ssq(block_sum_f64(s, s_sum, 4), H, p.eps);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (n[i] <= 0) continue;
+            if (p.post_w) {
+                float w[8];
+                load8<false, VEC>(p.post_w, c0[i], n[i], w);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) u[i][c] = u[i][c] * post * w[c];
+            }
+            if (p.gate) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    u[i][c] = u[i][c] / (1.0f + expf(-g[i][c]));
+                    if (p.gate_act == kGateSilu) u[i][c] *= g[i][c];
+                }
+            }
+            float sc[8];
+            if (p.scale_v) {
+                load8<false, VEC>(p.scale_v, c0[i], n[i], sc);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) sc[c] = p.scale;
+            }
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[i][c] += sc[c] * u[i][c];
+            store8<BF16, VEC>(p.x_out, row + c0[i], n[i], v[i]);
+        }
     }
     double s = 0.0;
-    for (int i = threadIdx.x; i < H; i += 256) {
-        float v = at(p.x, i);
-        if (p.y) {
-            float u = at(p.y, i);
-            if (p.post_w) u = u * post * p.post_w[i];
-            if (p.gate) {
-                const float g = at(p.gate, i);
-                u = u / (1.0f + expf(-g));
-                if (p.gate_act == kGateSilu) u *= g;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) s += (double)(v[i][c] * v[i][c]);  // (columns past H are zeros)
+    float w[NP][8];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) w[i][c] = 1.0f;
+        if (p.w && n[i] > 0) load8<false, VEC>(p.w, c0[i], n[i], w[i]);
+    }
+    const float r = rms_scale_from_ssq(block_sum_f64(s, s_sum[1]), H, p.eps);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[i][c] = v[i][c] * r * w[i][c];
+        if (n[i] > 0) store8<BF16, VEC>(p.h, row + c0[i], n[i], v[i]);
+        if (p.q) {
+            float inv;
+            const float m = fp8_block_max(v[i], inv);
+            uint32_t o[2];
+            fp8_pack8(v[i], inv, o);
+            if (n[i] > 0) {
+                if (VEC) {
+                    *(uint2*)(p.q + row + c0[i]) = make_uint2(o[0], o[1]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < n[i]) p.q[row + c0[i] + c] = (uint8_t)(o[c >> 2] >> (8 * (c & 3)));
+                }
+                const int nb = (H + kFp8Block - 1) / kFp8Block;
+                if ((threadIdx.x & 15) == 0) p.q_scale[(uint64_t)blockIdx.x * nb + c0[i] / kFp8Block] = m / kFp8Max;
             }
-            v += (p.scale_v ? p.scale_v[i] : p.scale) * u;
-            put(p.x_out, i, v);
         }
-        s_row[i] = v;
-        s += (double)(v * v);
     }
-    const float r = rms_scale_from_ssq(block_sum_f64(s, s_sum, 4), H, p.eps);
-    for (int i = threadIdx.x; i < H; i += 256) {
-        float v = s_row[i] * r;
-        if (p.w) v *= p.w[i];
-        s_row[i] = v;
-        put(p.h, i, v);
-    }
-    if (!p.q) return;
-    __syncthreads();
-    const int nb = (H + kFp8Block - 1) / kFp8Block;
-    for (int b = threadIdx.x >> 4; b < nb; b += 16) {
-        const int c0 = b * kFp8Block + 8 * ((int)threadIdx.x & 15);
-        float v[8], inv;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c0 + i < H ? s_row[c0 + i] : 0.0f;
-        const float m = fp8_block_max(v, inv);
-        uint32_t o[2];
-        fp8_pack8(v, inv, o);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c0 + i < H) p.q[row + c0 + i] = (uint8_t)(o[i >> 2] >> (8 * (i & 3)));
-        if ((threadIdx.x & 15) == 0) p.q_scale[(uint64_t)blockIdx.x * nb + b] = m / kFp8Max;
-    }
+}
+
+template <bool BF16, bool VEC>
+static void launch_norm(const ResidualNorm& p, int n_tokens, hipStream_t stream) {
+    const int pieces = (p.H + 7) / 8, np = pieces > 1024 ? 2 : 1;
+    const dim3 grid(n_tokens), block((unsigned)(((pieces + np - 1) / np + 63) / 64 * 64));
+    if (np == 2) hipLaunchKernelGGL((k_residual_norm<BF16, VEC, 2>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((k_residual_norm<BF16, VEC, 1>), grid, block, 0, stream, p);
 }
 
 hipError_t launch_residual_norm(const ResidualNorm& p, bool bf16, int n_tokens, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const size_t lds = (size_t)p.H * sizeof(float);
-    if (bf16) hipLaunchKernelGGL(k_residual_norm<true>, dim3(n_tokens), dim3(256), lds, stream, p);
-    else hipLaunchKernelGGL(k_residual_norm<false>, dim3(n_tokens), dim3(256), lds, stream, p);
+    if (p.H > 16384) return hipErrorInvalidValue;
+    const uintptr_t any = (uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.gate | (uintptr_t)p.post_w | (uintptr_t)p.scale_v |
+                          (uintptr_t)p.w | (uintptr_t)p.x_out | (uintptr_t)p.h | (uintptr_t)p.q;
+    const bool vec = p.H % 8 == 0 && (any & 15u) == 0;
+    if (bf16) { if (vec) launch_norm<true, true>(p, n_tokens, stream); else launch_norm<true, false>(p, n_tokens, stream); }
+    else { if (vec) launch_norm<false, true>(p, n_tokens, stream); else launch_norm<false, false>(p, n_tokens, stream); }
     return hipGetLastError();
 }
 

@@ -154,7 +154,7 @@ int qmoe_gather_tokens(const void* x, int32_t elem_bytes, int32_t n_tokens, int3
                        int32_t n_experts, const int32_t* offsets, const int32_t* place, void* y, void* hip_stream) {
     qmoe::clear_error();
     QMOE_TRY(check_tokens(n_tokens, top_k));
-    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 28));
+    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     QMOE_TRY(in_range("n_experts", n_experts, 1, 1024));
     if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return bad_value("elem_bytes", "1, 2 or 4", str(elem_bytes));
     if (n_tokens == 0) return QMOE_OK;
@@ -177,7 +177,7 @@ int qmoe_combine_tokens(const void* ys, int32_t x_type, int32_t n_tokens, int32_
     qmoe::clear_error();
     QMOE_TRY(row_type("x_type", x_type));
     QMOE_TRY(check_tokens(n_tokens, top_k));
-    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 28));
+    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     if (n_tokens == 0) return QMOE_OK;
     QMOE_TRY(need("ys", ys));
     QMOE_TRY(need("place", place));
@@ -199,7 +199,7 @@ int qmoe_combine_tokens_backward(const void* dy, const void* ys, int32_t x_type,
     qmoe::clear_error();
     QMOE_TRY(row_type("x_type", x_type));
     QMOE_TRY(check_tokens(n_tokens, top_k));
-    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 28));
+    QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     QMOE_TRY(in_range("n_experts", n_experts, 1, 1024));
     if (n_tokens == 0) return QMOE_OK;
     QMOE_TRY(need("dy", dy));

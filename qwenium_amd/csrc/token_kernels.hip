@@ -11,169 +11,251 @@ namespace qmoe {
 // offset) and its own -- and once more to write its own assignments in ascending
 // order, so no workgroup waits for another and the result does not depend on
 // their order.  Workgroup E takes the ids outside [0, E): place -1, and the list's
-// tail behind offsets[E] filled with -1.  The waves take contiguous quarters.
+// tail behind offsets[E] filled with -1.  The waves take contiguous shares, 4 ids a
+// lane and step.
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void k_sort_tokens(const int32_t* ids, int A, int top_k, int E, int32_t* offsets,
-                                                     int32_t* rows, int32_t* tokens, int32_t* place) {
-    __shared__ int s_below[4], s_own[4];
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void k_sort_tokens(const int32_t* ids, int A, int top_k, int E, bool vec,
+                                                         int32_t* offsets, int32_t* rows, int32_t* tokens, int32_t* place) {
+    __shared__ int s_below[NW], s_own[NW];
     const int e = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int quarter = ((A + 3) / 4 + 255) / 256 * 256;
-    const int64_t from = (int64_t)wave * quarter;
-    const int begin = from < A ? (int)from : A, end = A - begin < quarter ? A : begin + quarter;
+    const int64_t share = ((int64_t)A + 256 * NW - 1) / (256 * NW) * 256;
+    const int64_t begin = wave * share, end = begin + share < A ? begin + share : A;
+    auto load4 = [&](int64_t a, int (&id)[4]) {  // E + 1 marks what does not exist
+        if (vec && a + 4 <= end) {
+            const u32x4 r = *(const u32x4*)(ids + a);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) id[c] = (uint32_t)r[c] < (uint32_t)E ? (int)r[c] : E;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = a + c < end ? ids[a + c] : 0;
+                id[c] = a + c >= end ? E + 1 : (uint32_t)r < (uint32_t)E ? r : E;
+            }
+        }
+    };
     int below = 0, own = 0;
-    for (int a = begin + lane; a < end; a += 64) {
-        const int id = ids[a];
-        const bool valid = id >= 0 && id < E;
-        below += valid && id < e;
-        own += e < E ? id == e : !valid;
+#pragma unroll 4
+    for (int64_t a0 = begin; a0 < end; a0 += 256) {
+        int id[4];
+        load4(a0 + 4 * lane, id);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            below += id[c] < e;
+            own += id[c] == e;
+        }
     }
     below = group_sum_i32<64>(below);
     own = group_sum_i32<64>(own);
     if (lane == 0) s_below[wave] = below, s_own[wave] = own;
     __syncthreads();
-    int at = s_below[0] + s_below[1] + s_below[2] + s_below[3];
-    if (threadIdx.x == 0) offsets[e] = at;
-    for (int w = 0; w < wave; ++w) at += s_own[w];
-    for (int a0 = begin; a0 < end; a0 += 64) {
-        const int a = a0 + lane;
-        const int id = a < end ? ids[a] : 0;
-        const bool mine = a < end && (e < E ? id == e : id < 0 || id >= E);
-        const uint64_t mask = __ballot(mine);
-        if (mine) {
-            const int pos = at + __builtin_popcountll(mask & ((1ull << lane) - 1));
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        at += s_below[w];
+        if (w < wave) at += s_own[w];
+    }
+    if (threadIdx.x == 0) offsets[e] = at;  // (wave 0: no own counts in it)
+    if (own == 0) return;
+#pragma unroll 4
+    for (int64_t a0 = begin; a0 < end; a0 += 256) {
+        int id[4];
+        load4(a0 + 4 * lane, id);
+        const uint64_t lower = (1ull << lane) - 1;
+        int before = 0, all = 0;  // own ids of the lanes below; of the wave
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint64_t mask = __ballot(id[c] == e);
+            before += __builtin_popcountll(mask & lower);
+            all += __builtin_popcountll(mask);
+        }
+        int pos = at + before;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (id[c] != e) continue;
+            const int a = (int)(a0 + 4 * lane + c);
             rows[pos] = e < E ? a : -1;
             tokens[pos] = e < E ? a / top_k : -1;
             place[a] = e < E ? pos : -1;
+            ++pos;
         }
-        at += __builtin_popcountll(mask);
+        at += all;
     }
 }
 
 hipError_t launch_sort_tokens(const int32_t* ids, int n_tokens, int top_k, int E, int32_t* offsets, int32_t* rows,
                               int32_t* tokens, int32_t* place, hipStream_t stream) {
-    hipLaunchKernelGGL(k_sort_tokens, dim3(E + 1), dim3(256), 0, stream, ids, n_tokens * top_k, top_k, E, offsets, rows,
-                       tokens, place);
+    const int A = n_tokens * top_k;
+    const bool vec = ((uintptr_t)ids & 15u) == 0;
+    if (A <= 1024)
+        hipLaunchKernelGGL(k_sort_tokens<4>, dim3(E + 1), dim3(256), 0, stream, ids, A, top_k, E, vec, offsets, rows, tokens,
+                           place);
+    else
+        hipLaunchKernelGGL(k_sort_tokens<16>, dim3(E + 1), dim3(1024), 0, stream, ids, A, top_k, E, vec, offsets, rows, tokens,
+                           place);
     return hipGetLastError();
 }
 
+// A token's row in pieces of 8 elements over threads x workgroups: workgroups of one
+// wave where wider ones would leave CUs without any.
+static void row_grid(int n_tokens, int64_t pieces, dim3& grid, dim3& block) {
+    const int64_t threads = n_tokens * ((pieces + 255) / 256) >= 512 ? 256 : 64;
+    grid = dim3((unsigned)n_tokens, (unsigned)((pieces + threads - 1) / threads));
+    block = dim3((unsigned)threads);
+}
+
 // ---------------------------------------------------------------------------
-// Rows to the experts' order: one workgroup per token reads its row once and
-// writes it top_k times (reading by sorted row would read it top_k times).  Rows
-// behind the last expert's belong to no token: zeros, by the workgroup that owns
-// those list indices.  Pieces of 16 bytes (V = u32x4) or single elements.
+// Rows to the experts' order: a token's workgroups read its row once and write it
+// top_k times (reading by sorted row would read it top_k times).  Rows behind the
+// last expert's belong to no token: zeros, by the token with those list indices.
+// Pieces of 16 bytes (V = u32x4) or single elements.
 // ---------------------------------------------------------------------------
 template <typename V>
 __global__ __launch_bounds__(256) void k_gather_tokens(const V* x, int n, int top_k, int R, const int32_t* total,
                                                        const int32_t* place, V* y) {
-    const int t = blockIdx.x;
-    const V* xr = x + (uint64_t)t * n;
+    const int t = blockIdx.x, i = blockIdx.y * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const V v = x[(uint64_t)t * n + i];
     const int32_t* pl = place + (int64_t)t * top_k;
     const int last = *total;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const V v = xr[i];
-        for (int j = 0; j < top_k; ++j) {
-            const int p = pl[j];
-            if (p >= 0 && p < R) y[(uint64_t)p * n + i] = v;
-            const int r = t * top_k + j;
-            if (r >= last) y[(uint64_t)r * n + i] = V{};
-        }
+#pragma unroll 4
+    for (int j = 0; j < top_k; ++j) {
+        const int p = pl[j];
+        if (p >= 0 && p < R) y[(uint64_t)p * n + i] = v;
+        const int r = t * top_k + j;
+        if (r >= last) y[(uint64_t)r * n + i] = V{};
     }
+}
+
+template <typename V>
+static hipError_t launch_gather(const void* x, int64_t n, int n_tokens, int top_k, const int32_t* total, const int32_t* place,
+                                void* y, hipStream_t stream) {
+    dim3 grid, block;
+    row_grid(n_tokens, n, grid, block);
+    if (grid.y > 65535) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_gather_tokens<V>, grid, block, 0, stream, (const V*)x, (int)n, top_k, n_tokens * top_k, total, place,
+                       (V*)y);
+    return hipGetLastError();
 }
 
 hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_cols, int top_k, const int32_t* total,
                                 const int32_t* place, void* y, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const int R = n_tokens * top_k;
     const int64_t bytes = (int64_t)n_cols * elem;
-    const dim3 grid(n_tokens), block(256);
     if (bytes % 16 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15u) == 0)
-        hipLaunchKernelGGL(k_gather_tokens<u32x4>, grid, block, 0, stream, (const u32x4*)x, (int)(bytes / 16), top_k, R, total,
-                           place, (u32x4*)y);
-    else if (elem == 4)
-        hipLaunchKernelGGL(k_gather_tokens<uint32_t>, grid, block, 0, stream, (const uint32_t*)x, n_cols, top_k, R, total,
-                           place, (uint32_t*)y);
-    else if (elem == 2)
-        hipLaunchKernelGGL(k_gather_tokens<uint16_t>, grid, block, 0, stream, (const uint16_t*)x, n_cols, top_k, R, total,
-                           place, (uint16_t*)y);
-    else
-        hipLaunchKernelGGL(k_gather_tokens<uint8_t>, grid, block, 0, stream, (const uint8_t*)x, n_cols, top_k, R, total,
-                           place, (uint8_t*)y);
-    return hipGetLastError();
+        return launch_gather<u32x4>(x, bytes / 16, n_tokens, top_k, total, place, y, stream);
+    if (elem == 4) return launch_gather<uint32_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
+    if (elem == 2) return launch_gather<uint16_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
+    return launch_gather<uint8_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
 }
 
 // ---------------------------------------------------------------------------
 // y[t] = residual[t] + sum_j w[t][j] ys[place[t][j]], j in order in f32, rounded
-// once (w null: ones, the gather's gradient).  Assignments without a place add nothing.
+// once (w null: ones, the gather's gradient).  Assignments without a place add
+// nothing.  8 columns a thread, the rows of 8 assignments in flight.
 // ---------------------------------------------------------------------------
-template <bool BF16>
-__device__ __forceinline__ float load1(const void* x, uint64_t at) {
-    return BF16 ? bf16_to_f32(((const uint16_t*)x)[at]) : ((const float*)x)[at];
-}
-template <bool BF16>
-__device__ __forceinline__ void store1(void* y, uint64_t at, float v) {
-    if (BF16) ((uint16_t*)y)[at] = (uint16_t)f32_pack_bf16(v, 0.0f);
-    else ((float*)y)[at] = v;
-}
-
-template <bool BF16>
+template <bool BF16, bool VEC>
 __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, int top_k, int R, const int32_t* place,
                                                         const float* w, const void* residual, void* y) {
-    const int t = blockIdx.x;
-    for (int i = threadIdx.x; i < H; i += 256) {
-        float s = 0.0f;
-        for (int j = 0; j < top_k; ++j) {
-            const int p = place[(int64_t)t * top_k + j];
-            if (p < 0 || p >= R) continue;
-            const float v = load1<BF16>(ys, (uint64_t)p * H + i);
-            s = w ? fmaf(w[(int64_t)t * top_k + j], v, s) : s + v;
+    const int t = blockIdx.x, c0 = 8 * (blockIdx.y * blockDim.x + threadIdx.x), n = H - c0;
+    if (n <= 0) return;
+    float s[8] = {}, res[8] = {};
+    if (residual) load8<BF16, VEC>(residual, (uint64_t)t * H + c0, n, res);
+    for (int j0 = 0; j0 < top_k; j0 += 8) {
+        float v[8][8], wj[8];
+        bool has[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int a = t * top_k + (j0 + j < top_k ? j0 + j : 0);
+            const int p = place[a];
+            has[j] = j0 + j < top_k && p >= 0 && p < R;
+            wj[j] = w ? w[a] : 1.0f;
+            if (has[j]) load8<BF16, VEC>(ys, (uint64_t)p * H + c0, n, v[j]);
         }
-        if (residual) s += load1<BF16>(residual, (uint64_t)t * H + i);
-        store1<BF16>(y, (uint64_t)t * H + i, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (has[j])
+#pragma unroll
+                for (int c = 0; c < 8; ++c) s[c] = fmaf(wj[j], v[j][c], s[c]);
     }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) s[c] += res[c];
+    store8<BF16, VEC>(y, (uint64_t)t * H + c0, n, s);
 }
 
 hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H, int top_k, const int32_t* place,
                                  const float* w, const void* residual, void* y, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    if (bf16)
-        hipLaunchKernelGGL(k_combine_tokens<true>, dim3(n_tokens), dim3(256), 0, stream, ys, H, top_k, n_tokens * top_k, place,
-                           w, residual, y);
-    else
-        hipLaunchKernelGGL(k_combine_tokens<false>, dim3(n_tokens), dim3(256), 0, stream, ys, H, top_k, n_tokens * top_k, place,
-                           w, residual, y);
+    const bool vec = H % 8 == 0 && (((uintptr_t)ys | (uintptr_t)residual | (uintptr_t)y) & 15u) == 0;
+    dim3 grid, block;
+    row_grid(n_tokens, ((int64_t)H + 7) / 8, grid, block);
+    if (grid.y > 65535) return hipErrorInvalidValue;
+#define QMOE_COMBINE(B, V) \
+    hipLaunchKernelGGL((k_combine_tokens<B, V>), grid, block, 0, stream, ys, H, top_k, n_tokens * top_k, place, w, residual, y)
+    if (bf16) { if (vec) QMOE_COMBINE(true, true); else QMOE_COMBINE(true, false); }
+    else { if (vec) QMOE_COMBINE(false, true); else QMOE_COMBINE(false, false); }
+#undef QMOE_COMBINE
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
 // The weighted sum's gradients: dys[place[t][j]] = w[t][j] dy[t] and
 // dw[t][j] = <dy[t], ys[place[t][j]]>.  One workgroup per token, so no sum is
-// shared between workgroups.  Rows behind the last expert's get zeros.
+// shared between workgroups: a thread adds its columns' products in turn (8
+// columns and 8 assignments in flight), then the tree over its wave's lanes and
+// the waves in turn.  Rows behind the last expert's get zeros.
 // ---------------------------------------------------------------------------
-template <bool BF16>
-__global__ __launch_bounds__(256) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
-                                                            const int32_t* total, const int32_t* place, const float* w,
-                                                            void* dys, float* dw) {
-    __shared__ float s_sum[4];
-    const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+template <bool BF16, bool VEC>
+__global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
+                                                             const int32_t* total, const int32_t* place, const float* w,
+                                                             void* dys, float* dw) {
+    __shared__ float s_sum[8][16];
+    const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, nw = blockDim.x >> 6;
     const int last = *total;
-    for (int j = 0; j < top_k; ++j) {
-        const int a = t * top_k + j, p = place[a];
-        float dot = 0.0f;
-        if (p >= 0 && p < R) {
-            const float wj = w[a];
-            for (int i = threadIdx.x; i < H; i += 256) {
-                const float g = load1<BF16>(dy, (uint64_t)t * H + i);
-                dot = fmaf(g, load1<BF16>(ys, (uint64_t)p * H + i), dot);
-                store1<BF16>(dys, (uint64_t)p * H + i, wj * g);
+    for (int j0 = 0; j0 < top_k; j0 += 8) {
+        float dot[8] = {};
+        for (int c0 = 8 * threadIdx.x; c0 < H; c0 += 8 * blockDim.x) {
+            const int n = H - c0;
+            float g[8], v[8][8];
+            load8<BF16, VEC>(dy, (uint64_t)t * H + c0, n, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int p = j0 + j < top_k ? place[t * top_k + j0 + j] : -1;
+                if (p >= 0 && p < R) load8<BF16, VEC>(ys, (uint64_t)p * H + c0, n, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j0 + j >= top_k) continue;
+                const int a = t * top_k + j0 + j, p = place[a];
+                float o[8];
+                if (p >= 0 && p < R) {
+                    const float wj = w[a];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        dot[j] = fmaf(g[c], v[j][c], dot[j]);
+                        o[c] = wj * g[c];
+                    }
+                    store8<BF16, VEC>(dys, (uint64_t)p * H + c0, n, o);
+                }
+                if (a >= last) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) o[c] = 0.0f;
+                    store8<BF16, VEC>(dys, (uint64_t)a * H + c0, n, o);
+                }
             }
         }
-        if (a >= last)
-            for (int i = threadIdx.x; i < H; i += 256) store1<BF16>(dys, (uint64_t)a * H + i, 0.0f);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-        if (lane == 0) s_sum[wave] = dot;
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) dot[j] += __shfl_xor(dot[j], o, 64);
+            if (lane == 0) s_sum[j][wave] = dot[j];
+        }
         __syncthreads();
-        if (threadIdx.x == 0) dw[a] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        if (threadIdx.x < 8 && j0 + (int)threadIdx.x < top_k) {
+            float s = 0.0f;
+            for (int i = 0; i < nw; ++i) s += s_sum[threadIdx.x][i];
+            dw[t * top_k + j0 + (int)threadIdx.x] = s;
+        }
         __syncthreads();
     }
 }
@@ -182,12 +264,15 @@ hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, 
                                      const int32_t* total, const int32_t* place, const float* w, void* dys, float* dw,
                                      hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    if (bf16)
-        hipLaunchKernelGGL(k_combine_tokens_bwd<true>, dim3(n_tokens), dim3(256), 0, stream, dy, ys, H, top_k,
-                           n_tokens * top_k, total, place, w, dys, dw);
-    else
-        hipLaunchKernelGGL(k_combine_tokens_bwd<false>, dim3(n_tokens), dim3(256), 0, stream, dy, ys, H, top_k,
-                           n_tokens * top_k, total, place, w, dys, dw);
+    const bool vec = H % 8 == 0 && (((uintptr_t)dy | (uintptr_t)ys | (uintptr_t)dys) & 15u) == 0;
+    const int64_t pieces = ((int64_t)H + 7) / 8;
+    const dim3 grid(n_tokens), block((unsigned)(pieces < 1024 ? (pieces + 63) / 64 * 64 : 1024));
+#define QMOE_BWD(B, V)                                                                                                \
+    hipLaunchKernelGGL((k_combine_tokens_bwd<B, V>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, place, w, \
+                       dys, dw)
+    if (bf16) { if (vec) QMOE_BWD(true, true); else QMOE_BWD(true, false); }
+    else { if (vec) QMOE_BWD(false, true); else QMOE_BWD(false, false); }
+#undef QMOE_BWD
     return hipGetLastError();
 }
 
