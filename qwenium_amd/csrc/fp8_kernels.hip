@@ -11,6 +11,7 @@ namespace qmoe {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
@@ -98,12 +99,14 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Tile g of the list "experts in order, each with ceil(rows / tile) tiles" (a wave
-// finds it by itself, 256 experts a step).  Offsets outside [0, R] are taken as its ends.
-__device__ __forceinline__ bool fp8_find_tile(const Fp8Product& p, int tile, int g, int& expert, int& row0, int& end) {
+// finds it by itself, 256 experts a step); once: its expert has no other.  Offsets outside [0, R] are taken as its ends.
+__device__ __forceinline__ bool fp8_find_tile(const Fp8Product& p, int tile, int g, int& expert, int& row0, int& end,
+                                              bool& once) {
     if (!p.offsets) {
         expert = 0;
         row0 = g * tile;
         end = p.R;
+        once = false;
         return row0 < p.R;
     }
     const int lane = threadIdx.x & 63;
@@ -127,6 +130,7 @@ __device__ __forceinline__ bool fp8_find_tile(const Fp8Product& p, int tile, int
                 expert = c + 64 * j + at;
                 row0 = __builtin_amdgcn_readlane(l, at) + (g - base - __builtin_amdgcn_readlane(incl - t, at)) * tile;
                 end = __builtin_amdgcn_readlane(h, at);
+                once = __builtin_amdgcn_readlane(t, at) == 1;
                 return true;
             }
             base += total;
@@ -162,33 +166,33 @@ __device__ __forceinline__ int fp8_source_row(const Fp8Product& p, int r) {
 }
 
 // C consecutive columns (4 or 8) of a row from column n on; those past N are left out.
+template <typename V>
+__device__ __forceinline__ void fp8_put(const Fp8Product& p, void* y, V v) {
+    if (p.stream_out) {
+        asm volatile("");  // (keeps the two stores apart: merged ones lose the hint)
+        __builtin_nontemporal_store(v, (V*)y);
+        asm volatile("");
+    } else {
+        *(V*)y = v;
+    }
+}
 template <bool BF16, int C>
 __device__ __forceinline__ void fp8_store(const Fp8Product& p, int r, int n, const float (&v)[C]) {
+    static_assert(C == 4 || (C == 8 && BF16), "up to 16 bytes");
     const uint64_t at = (uint64_t)r * p.N + n;
     if (p.vec_out && n + C <= p.N) {
-        if constexpr (BF16) {
-            uint32_t o[C / 2];
-#pragma unroll
-            for (int i = 0; i < C / 2; ++i) o[i] = f32_pack_bf16(v[2 * i], v[2 * i + 1]);
-            if constexpr (C == 4) {
-                *(uint2*)((uint16_t*)p.y + at) = make_uint2(o[0], o[1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < C / 8; ++i)
-                    *(u32x4*)((uint16_t*)p.y + at + 8 * i) = u32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
-            }
+        if constexpr (!BF16) {
+            fp8_put(p, (float*)p.y + at, f32x4{v[0], v[1], v[2], v[3]});
+        } else if constexpr (C == 4) {
+            fp8_put(p, (uint16_t*)p.y + at, u32x2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3])});
         } else {
-#pragma unroll
-            for (int i = 0; i < C / 4; ++i)
-                *(f32x4*)((float*)p.y + at + 4 * i) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            fp8_put(p, (uint16_t*)p.y + at, u32x4{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
+                                                  f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])});
         }
     } else {
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            if (n + i < p.N) {
-                if (BF16) ((uint16_t*)p.y)[at + i] = (uint16_t)f32_pack_bf16(v[i], 0.0f);
-                else ((float*)p.y)[at + i] = v[i];
-            }
+            if (n + i < p.N) store1<BF16>(p.y, at + i, v[i]);
     }
 }
 
@@ -210,7 +214,8 @@ __global__ __launch_bounds__(256) void k_fp8_stream(Fp8Product p) {
     const int nt = (p.N + 15) >> 4;
     const int tile = blockIdx.x / nt, n0 = (blockIdx.x - tile * nt) * 16;
     int e, row0, end;
-    if (!fp8_find_tile(p, 16 * MT, tile, e, row0, end)) return;
+    bool once;
+    if (!fp8_find_tile(p, 16 * MT, tile, e, row0, end, once)) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4;
     const int KB = p.KB;
     const int n = n0 + (lane & 15);
@@ -332,9 +337,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     extern __shared__ uint8_t s_dyn[];
     const int nt = (p.N + T::kBN - 1) / T::kBN;
     int tile, n0, e, row0, end;
+    bool once;
     fp8_place(p, T::kBM, nt, tile, n0);
     n0 *= T::kBN;
-    if (!fp8_find_tile(p, T::kBM, tile, e, row0, end)) return;
+    if (!fp8_find_tile(p, T::kBM, tile, e, row0, end, once)) return;
+    // Weights that this row tile alone reads, in whole 128-byte lines, go past the caches.  256 experts of
+    // 1024 x 2048, four layers' weights in turn, us without and with: 80 rows 33.0 / 29.5, 512 rows 83 / 69,
+    // 4096 96 / 90, 32768 151 / 148; with two tiles an expert (128 of 1408 x 2816, 32768 rows) 225 / 266;
+    // with 5.5 lines a row (128 of 2816 x 704, 1688 rows) 58 / 64.
+    once = once && p.K % kFp8Block == 0;
     const int nrows = end - row0 < T::kBM ? end - row0 : T::kBM;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave % WM, wn = wave / WM;
@@ -379,7 +390,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
         const int at = c < p.K ? c : p.K - 16;  // past K: any valid piece, its weights are zeroed below
         const uint32_t base = lds0 + buf * T::kStage;
         if (l < kGA) dma_lds16_at(ga[l] + at, base + 1024 * group_a(l));
-        else dma_lds16(wt, gw[l - kGA] + (uint32_t)at, base + T::kBM * kFp8Block + 1024 * (wave + T::kWaves * (l - kGA)));
+        else {
+            const uint32_t to = base + T::kBM * kFp8Block + 1024 * (wave + T::kWaves * (l - kGA));
+            if (once) dma_lds16<true>(wt, gw[l - kGA] + (uint32_t)at, to);
+            else dma_lds16<false>(wt, gw[l - kGA] + (uint32_t)at, to);
+        }
     };
     // The row scales of steps b .. b + 3, by the waves 0 .. kScaleLoads - 1: 64 rows each, 16 bytes a row
     // (a row's scales lie KB apart: one 64-row load of single scales costs as much).  Where KB is no
@@ -487,7 +502,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
                     for (int l = 0; l < T::kLoads; ++l)
                         if (ST == 2 ? i == 0 : l >= i * T::kLoads / MI && l < (i + 1) * T::kLoads / MI) load(l, b + ST - 1, next);
                 }
-                __builtin_amdgcn_sched_barrier(0);
+                if (!BF16) __builtin_amdgcn_sched_barrier(0);  // (loads moved up from the next subtile would spill)
             }
             buf = buf + 1 == ST ? 0 : buf + 1;
             next = next + 1 == ST ? 0 : next + 1;
@@ -572,21 +587,24 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         // 1024 58 / 35 / 27 / 37, 256 56 / 34 / 19 / 17.
         if (wgs(256, 256) >= kFp8Cus) return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
-    } else {
-        // By the rows an expert has on average: the tile that holds most experts' rows with few rows to
-        // spare.  256 experts of 1024 x 2048, bf16, us with 256x256 / 160x128 / 128x256 / 64x128: 32 rows
-        // 123 / 107 / 104 / 99, 64 rows 133 / 121 / 114 / 125, 128 rows 153 / 158 / 154 / 194, 187 rows
-        // 182 / 210 / 204 / 259; 128 experts of 2816 x 704: 125 rows 109 / 99 / 109 / 118; f32, 128 rows
-        // 240 / 206 / 222 / 241.
-        const int64_t mean = p.R / p.E;
-        if (mean >= 110) {
-            const int64_t most = mean + mean / 7;  // (most experts' rows, evenly drawn)
-            if ((most + 255) / 256 * 256 < (most + 159) / 160 * 160 && wgs(256, 256) >= kFp8Cus)
-                return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
-            if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
-        } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
-            return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
-        }
+        if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
+        return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
+    }
+    // By the rows an expert has on average: the tile that holds most experts' rows with few rows to
+    // spare.  256 experts of 1024 x 2048, bf16, us with 256x256 / 160x128 / 128x256 / 64x128: 32 rows
+    // 123 / 107 / 104 / 99, 64 rows 133 / 121 / 114 / 125, 128 rows 153 / 158 / 154 / 194, 187 rows
+    // 182 / 210 / 204 / 259; 128 experts of 2816 x 704: 125 rows 109 / 99 / 109 / 118; f32, 128 rows
+    // 240 / 206 / 222 / 241 (all with weights and results through the caches).
+    const int64_t mean = p.R / p.E, most = mean + mean / 7;  // (most experts' rows, evenly drawn)
+    // bf16 results larger than an L2 past the caches where the weights go past them: 32768 rows 150 / 142 us,
+    // 4096 rows (8 MB) 89 / 85, the quantization after them no slower; 512 rows (1 MB) 69 / 72; f32 197 / 201.
+    p.stream_out = bf16 && most <= 256 && (int64_t)p.R * p.N * 2 > (4 << 20);
+    if (mean >= 110) {
+        if ((most + 255) / 256 * 256 < (most + 159) / 160 * 160 && wgs(256, 256) >= kFp8Cus)
+            return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
+        if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
+    } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
+        return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
     }
     if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
     return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);

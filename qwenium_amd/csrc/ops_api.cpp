@@ -50,7 +50,7 @@ int done(hipError_t err, const char* what) { return err == hipSuccess ? QMOE_OK 
 int check_tokens(int32_t n_tokens, int32_t top_k) {
     if (int rc = in_range("n_tokens", n_tokens, 0, INT32_MAX)) return rc;
     if (int rc = in_range("top_k", top_k, 1, 64)) return rc;
-    return in_range("n_tokens * top_k", (int64_t)n_tokens * top_k, 0, INT32_MAX);
+    return in_range("n_tokens * top_k", (int64_t)n_tokens * top_k, 0, 1 << 30);
 }
 
 #define QMOE_TRY(expr)                   \

@@ -306,9 +306,15 @@ __device__ __forceinline__ double dpp_sum_f64(double v) {
 // for them itself (s_waitcnt vmcnt at the chunk boundary, then a barrier).
 // M0 takes the LDS base; the LDS-DMA read of M0 needs one wait state.
 // Source: a wave-uniform base plus this lane's 32-bit byte offset.
+// NT: not kept in the caches.
+template <bool NT = false>
 __device__ __forceinline__ void dma_lds16(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-                 : "memory", "m0");
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "s"(lds)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+                     : "memory", "m0");
 }
 __device__ __forceinline__ void dma_lds4(const void* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds)

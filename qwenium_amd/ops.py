@@ -331,8 +331,8 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor], w: Optional[torch.
         for name, v in (("w", w), ("post_w", post_w), ("scale", scale if vector else None)):
             if v is not None:
                 _kept(name, v, dev, (H,), torch.float32)
-        x_out = x if y is None else _out("out", out, dev, (T, H), dt)
-        h = torch.empty((T, H), dtype=dt, device=dev)
+        x_out = x if y is None else torch.empty_like(x) if out is None else _kept("out", out, dev, (T, H), dt)
+        h = torch.empty_like(x)
         q = q_scale = None
         if quantize:
             q = torch.empty((T, H), dtype=FP8, device=dev)
