@@ -221,6 +221,23 @@ __global__ __launch_bounds__(256) void k_fp8_stream(Fp8Product p) {
     const int n = n0 + (lane & 15);
     const uint8_t* wr = p.w + ((uint64_t)e * p.N + (n < p.N ? n : p.N - 1)) * p.K;
     const float* sw = p.sw + ((uint64_t)e * p.NB + (n0 >> 7)) * KB;
+    // past the end: the last block again, scaled by zero
+    auto block = [&](int b0, int u) { return b0 + 4 * u < KB ? b0 + 4 * u : KB - 1; };
+    auto piece = [&](int b, int h) {
+        const int c = b * kFp8Block + 16 * (g + 4 * h);
+        return c < p.K ? c : p.K - 16;
+    };
+    i32x4 wv[U][2];
+    float ws[U];
+    auto load_w = [&](int b0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) wv[u][h] = *(const i32x4*)(wr + piece(block(b0, u), h));
+            ws[u] = sw[block(b0, u)];
+        }
+    };
+    load_w(wave < KB ? wave : KB - 1);  // the first weights are on their way while the rows' indices come
     const uint8_t* ar[MT];
     const float* sa[MT];
     int src[MT];
@@ -234,23 +251,18 @@ __global__ __launch_bounds__(256) void k_fp8_stream(Fp8Product p) {
     }
     f32x4 acc[MT] = {};
     for (int b0 = wave; b0 < KB; b0 += 4 * U) {
-        i32x4 wv[U][2], av[U][MT][2];
-        float ws[U], as[U][MT];
+        i32x4 av[U][MT][2];
+        float as[U][MT];
+        if (b0 != wave) load_w(b0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            // past the end: the last block again, scaled by zero
-            const int b = b0 + 4 * u < KB ? b0 + 4 * u : KB - 1;
+            const int b = block(b0, u);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = b * kFp8Block + 16 * (g + 4 * h);
-                const int at = c < p.K ? c : p.K - 16;
-                wv[u][h] = *(const i32x4*)(wr + at);
+            for (int i = 0; i < MT; ++i) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) av[u][i][h] = *(const i32x4*)(ar[i] + at);
+                for (int h = 0; h < 2; ++h) av[u][i][h] = *(const i32x4*)(ar[i] + piece(b, h));
+                as[u][i] = sa[i][b];
             }
-            ws[u] = sw[b];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) as[u][i] = sa[i][b];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
