@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "qmoe_internal.h"
@@ -40,8 +41,24 @@ int row_type(const char* what, int32_t t) {
 
 unsigned elem(int32_t type) { return type == QMOE_TYPE_BF16 ? 2 : 4; }
 
-int distinct(const char* what, const void* p, const char* other, const void* q) {
-    return p != q || !p ? QMOE_OK : bad_value(what, std::string("a buffer distinct from ") + other, "the same address");
+// A buffer of the call: outputs overlap nothing else, except where a call takes the very same buffer.
+struct Buffer {
+    const char* name;
+    const void* at;
+    uint64_t bytes;
+    bool overlaps(const Buffer& o) const {
+        const uintptr_t p = (uintptr_t)at, q = (uintptr_t)o.at;
+        return at && o.at && p < q + o.bytes && q < p + bytes;
+    }
+};
+int apart(std::initializer_list<Buffer> outs, std::initializer_list<Buffer> ins) {
+    for (const Buffer* o = outs.begin(); o != outs.end(); ++o) {
+        for (const Buffer* r = outs.begin(); r != o; ++r)
+            if (o->overlaps(*r)) return bad_value(o->name, std::string("a buffer distinct from ") + r->name, "an overlapping one");
+        for (const Buffer& i : ins)
+            if (o->overlaps(i)) return bad_value(o->name, std::string("a buffer distinct from ") + i.name, "an overlapping one");
+    }
+    return QMOE_OK;
 }
 
 int done(hipError_t err, const char* what) { return err == hipSuccess ? QMOE_OK : qmoe::hip_error(err, what); }
@@ -76,8 +93,9 @@ int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_c
     QMOE_TRY(need("scale", scale));
     QMOE_TRY(aligned("x", x, elem(x_type)));
     QMOE_TRY(aligned("scale", scale, 4));
-    QMOE_TRY(distinct("q", q, "x", x));
-    QMOE_TRY(distinct("scale", scale, "x", x));
+    const uint64_t v = (uint64_t)n_rows * n_cols;
+    QMOE_TRY(apart({{"q", q, v}, {"scale", scale, 4 * (uint64_t)n_rows * ((n_cols + 127) / 128)}},
+                   {{"x", x, v * elem(x_type) * (act == QMOE_FP8_ACT_NONE ? 1 : 2)}}));
     return done(qmoe::launch_fp8_quantize(x, x_type == QMOE_TYPE_BF16, n_rows, n_cols, act, q, scale, (hipStream_t)hip_stream),
                 "fp8_quantize kernel");
 }
@@ -109,8 +127,10 @@ int qmoe_fp8_matmul(const uint8_t* a, const float* a_scale, int32_t a_rows, cons
     QMOE_TRY(aligned("offsets", offsets, 4));
     QMOE_TRY(aligned("rows", rows, 4));
     QMOE_TRY(aligned("y", y, elem(y_type)));
-    QMOE_TRY(distinct("y", y, "a", a));
-    QMOE_TRY(distinct("y", y, "w", w));
+    const uint64_t kb = (k + 127) / 128, nb = (n + 127) / 128, e = (uint64_t)n_experts;
+    QMOE_TRY(apart({{"y", y, (uint64_t)n_rows * n * elem(y_type)}},
+                   {{"a", a, (uint64_t)a_rows * k}, {"a_scale", a_scale, 4 * a_rows * kb}, {"w", w, e * n * k},
+                    {"w_scale", w_scale, 4 * e * nb * kb}, {"offsets", offsets, 4 * (e + 1)}, {"rows", rows, 4 * (uint64_t)n_rows}}));
     qmoe::Fp8Product p{};
     p.a = a;
     p.sa = a_scale;
@@ -143,7 +163,10 @@ int qmoe_sort_tokens(const int32_t* topk_idx, int32_t n_tokens, int32_t top_k, i
         QMOE_TRY(aligned("rows", rows, 4));
         QMOE_TRY(aligned("tokens", tokens, 4));
         QMOE_TRY(aligned("place", place, 4));
-        QMOE_TRY(distinct("place", place, "topk_idx", topk_idx));
+        const uint64_t list = 4 * (uint64_t)n_tokens * top_k;
+        QMOE_TRY(apart({{"offsets", offsets, 4 * ((uint64_t)n_experts + 1)}, {"rows", rows, list}, {"tokens", tokens, list},
+                        {"place", place, list}},
+                       {{"topk_idx", topk_idx, list}}));
     }
     return done(qmoe::launch_sort_tokens(topk_idx, n_tokens, top_k, n_experts, offsets, rows, tokens, place,
                                          (hipStream_t)hip_stream),
@@ -166,7 +189,9 @@ int qmoe_gather_tokens(const void* x, int32_t elem_bytes, int32_t n_tokens, int3
     QMOE_TRY(aligned("y", y, (unsigned)elem_bytes));
     QMOE_TRY(aligned("offsets", offsets, 4));
     QMOE_TRY(aligned("place", place, 4));
-    QMOE_TRY(distinct("y", y, "x", x));
+    const uint64_t row = (uint64_t)n_cols * elem_bytes, list = (uint64_t)n_tokens * top_k;
+    QMOE_TRY(apart({{"y", y, list * row}}, {{"x", x, n_tokens * row}, {"offsets", offsets, 4 * ((uint64_t)n_experts + 1)},
+                                             {"place", place, 4 * list}}));
     return done(qmoe::launch_gather_tokens(x, elem_bytes, n_tokens, n_cols, top_k, offsets + n_experts, place, y,
                                            (hipStream_t)hip_stream),
                 "gather_tokens kernel");
@@ -187,7 +212,9 @@ int qmoe_combine_tokens(const void* ys, int32_t x_type, int32_t n_tokens, int32_
     QMOE_TRY(aligned("y", y, elem(x_type)));
     QMOE_TRY(aligned("place", place, 4));
     QMOE_TRY(aligned("w", w, 4));
-    QMOE_TRY(distinct("y", y, "ys", ys));
+    const uint64_t row = (uint64_t)n_cols * elem(x_type), list = (uint64_t)n_tokens * top_k;
+    QMOE_TRY(apart({{"y", y, n_tokens * row}}, {{"ys", ys, list * row}, {"place", place, 4 * list}, {"w", w, 4 * list},
+                                                 {"residual", residual == y ? nullptr : residual, n_tokens * row}}));
     return done(qmoe::launch_combine_tokens(ys, x_type == QMOE_TYPE_BF16, n_tokens, n_cols, top_k, place, w, residual, y,
                                             (hipStream_t)hip_stream),
                 "combine_tokens kernel");
@@ -216,9 +243,10 @@ int qmoe_combine_tokens_backward(const void* dy, const void* ys, int32_t x_type,
     QMOE_TRY(aligned("place", place, 4));
     QMOE_TRY(aligned("w", w, 4));
     QMOE_TRY(aligned("dw", dw, 4));
-    QMOE_TRY(distinct("dys", dys, "dy", dy));
-    QMOE_TRY(distinct("dys", dys, "ys", ys));
-    QMOE_TRY(distinct("dw", dw, "w", w));
+    const uint64_t row = (uint64_t)n_cols * elem(x_type), list = (uint64_t)n_tokens * top_k;
+    QMOE_TRY(apart({{"dys", dys, list * row}, {"dw", dw, 4 * list}},
+                   {{"dy", dy, n_tokens * row}, {"ys", ys, list * row}, {"offsets", offsets, 4 * ((uint64_t)n_experts + 1)},
+                    {"place", place, 4 * list}, {"w", w, 4 * list}}));
     return done(qmoe::launch_combine_tokens_bwd(dy, ys, x_type == QMOE_TYPE_BF16, n_tokens, n_cols, top_k,
                                                 offsets + n_experts, place, w, dys, dw, (hipStream_t)hip_stream),
                 "combine_tokens_backward kernel");
@@ -252,13 +280,14 @@ int qmoe_residual_norm(const qmoe_norm_args* a, int32_t n_tokens, int32_t n_embd
     QMOE_TRY(aligned("scale_v", a->scale_v, 4));
     QMOE_TRY(aligned("w", a->w, 4));
     QMOE_TRY(aligned("q_scale", a->q_scale, 4));
-    QMOE_TRY(distinct("h", a->h, "x", a->x));
-    QMOE_TRY(distinct("h", a->h, "y", a->y));
-    QMOE_TRY(distinct("h", a->h, "gate", a->gate));
-    QMOE_TRY(distinct("h", a->h, "x_out", a->x_out));
-    QMOE_TRY(distinct("x_out", a->x_out, "gate", a->gate));
-    QMOE_TRY(distinct("q", a->q, "h", a->h));
-    QMOE_TRY(distinct("q", a->q, "x", a->x));
+    const uint64_t v = (uint64_t)n_tokens * n_embd, vec = 4 * (uint64_t)n_embd;
+    auto other = [&](const void* in) { return in == a->x_out ? nullptr : in; };  // x' may replace x or y
+    const Buffer x{"x", a->x, v * e}, y{"y", a->y, v * e}, gate{"gate", a->gate, v * e}, post_w{"post_w", a->post_w, vec},
+        scale_v{"scale_v", a->scale_v, vec}, w{"w", a->w, vec};
+    QMOE_TRY(apart({{"x_out", a->y ? a->x_out : nullptr, v * e}},
+                   {{"x", other(a->x), v * e}, {"y", other(a->y), v * e}, gate, post_w, scale_v, w}));
+    QMOE_TRY(apart({{"h", a->h, v * e}, {"q", a->q, v}, {"q_scale", a->q_scale, 4 * (uint64_t)n_tokens * ((n_embd + 127) / 128)}},
+                   {x, y, gate, post_w, scale_v, w, {"x_out", a->y ? a->x_out : nullptr, v * e}}));
     qmoe::ResidualNorm p{};
     p.x = a->x;
     p.y = a->y;

@@ -118,6 +118,8 @@ def rc_quantize(x=FAKE, t=TYPE_F32, R=4, C=256, act=0, q=FAKE + MIB, s=FAKE + 2 
     (dict(C=0), QMOE_ERR_VALUE, "n_cols"), (dict(act=3), QMOE_ERR_VALUE, "act"), (dict(act=-1), QMOE_ERR_VALUE, "act"),
     (dict(x=None), QMOE_ERR_NULL, "x"), (dict(q=None), QMOE_ERR_NULL, "q"), (dict(s=None), QMOE_ERR_NULL, "scale"),
     (dict(x=FAKE + 2), QMOE_ERR_VALUE, "aligned"), (dict(q=FAKE), QMOE_ERR_VALUE, "distinct"),
+    (dict(q=FAKE + 4095), QMOE_ERR_VALUE, "q expected a buffer distinct from x"), (dict(s=FAKE - 28), QMOE_ERR_VALUE, "distinct"),
+    (dict(s=FAKE + MIB + 1020), QMOE_ERR_VALUE, "scale expected a buffer distinct from q"),
     (dict(R=2 ** 31 - 1, C=2 ** 28), QMOE_ERR_VALUE, "ceil(n_cols/128)"),
 ])
 def test_quantize_refusals(kw, code, needle):
@@ -150,7 +152,9 @@ def rc_matmul(a=FAKE, sa=FAKE + 0x100, A=4, w=FAKE + MIB, sw=FAKE + 2 * MIB, E=1
     (dict(w=None), QMOE_ERR_NULL, "w expected"), (dict(sw=None), QMOE_ERR_NULL, "w_scale"),
     (dict(y=None), QMOE_ERR_NULL, "y expected"), (dict(a=FAKE + 8), QMOE_ERR_VALUE, "16-byte"),
     (dict(w=FAKE + MIB + 4), QMOE_ERR_VALUE, "16-byte"), (dict(y=FAKE + MIB), QMOE_ERR_VALUE, "distinct"),
-    (dict(y=FAKE + MIB + 2), QMOE_ERR_VALUE, "aligned"),
+    (dict(y=FAKE + MIB + 2), QMOE_ERR_VALUE, "aligned"), (dict(y=FAKE + 508), QMOE_ERR_VALUE, "distinct from a"),
+    (dict(y=FAKE + MIB - 1020), QMOE_ERR_VALUE, "distinct from w"), (dict(R=2 ** 30 + 1, A=2 ** 30 + 1), QMOE_ERR_VALUE, "n_rows"),
+    (dict(offsets=FAKE + 3 * MIB + 1020), QMOE_ERR_VALUE, "distinct from offsets"),
 ])
 def test_matmul_refusals(kw, code, needle):
     assert rc_matmul(**kw) == code
@@ -192,7 +196,8 @@ def norm_args(**kw):
     (dict(gate_act=3), QMOE_ERR_VALUE, "gate_act"), (dict(y=None, post_w=FAKE), QMOE_ERR_VALUE, "y expected"),
     (dict(q=FAKE + 5 * MIB), QMOE_ERR_NULL, "q_scale"), (dict(eps=-1.0), QMOE_ERR_VALUE, "eps"),
     (dict(eps=float("nan")), QMOE_ERR_VALUE, "eps"), (dict(h=FAKE), QMOE_ERR_VALUE, "distinct"),
-    (dict(x_out=FAKE + 3 * MIB), QMOE_ERR_VALUE, "distinct"), (dict(h=FAKE + 2), QMOE_ERR_VALUE, "aligned"),
+    (dict(x_out=FAKE + 3 * MIB), QMOE_ERR_VALUE, "distinct"), (dict(x_out=FAKE + 1020), QMOE_ERR_VALUE, "distinct from x"),
+    (dict(w=FAKE + 3 * MIB + 1020), QMOE_ERR_VALUE, "distinct from w"), (dict(h=FAKE + 2), QMOE_ERR_VALUE, "aligned"),
 ])
 def test_norm_refusals(kw, code, needle):
     assert _lib.lib().qmoe_residual_norm(ctypes.byref(norm_args(**kw)), 4, 64, None) == code
@@ -211,6 +216,8 @@ def test_norm_width_refusals():
 def test_python_refuses_host_tensors():
     x = torch.zeros(4, 128)
     order = TokenOrder(*(torch.zeros(n, dtype=torch.int32) for n in (5, 8, 8)), torch.zeros(4, 2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="place expected"):
+        TokenOrder(order.offsets, order.rows, order.tokens, order.rows)
     with pytest.raises(ValueError, match="x expected a cuda"):
         qa.fp8_quantize(x)
     with pytest.raises(ValueError, match="act expected"):
@@ -415,18 +422,57 @@ def test_matmul_index_values(gpu, M):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M", [3, 150])
-def test_matmul_nan_stays_in_its_row(gpu, M):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [3, 150, 1500])
+def test_matmul_nan_stays_in_its_row(gpu, M, dtype):
     g = gen(7)
     a, s = fp8_rows(g, M, 144)
     w, sw = fp8_weights(g, 72, 144)
     a.view(torch.uint8)[1, 143] = 0x7F  # a NaN in the last, short block
     s2 = s.clone()
     s2[2, 0] = math.inf
-    y = qa.fp8_matmul(a.to(gpu), s2.to(gpu), w.to(gpu), sw.to(gpu)).cpu()
+    y = qa.fp8_matmul(a.to(gpu), s2.to(gpu), w.to(gpu), sw.to(gpu), out_dtype=dtype).cpu()
     assert torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any()
     keep = [i for i in range(M) if i not in (1, 2)]
-    check_product(y[keep], a[keep], s[keep], w, sw, torch.float32)
+    check_product(y[keep], a[keep], s[keep], w, sw, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E,R,N,K", [(0, 4100, 4104, 144), (0, 2050, 4100, 272), (0, 600, 2100, 528), (0, 300, 520, 144),
+                                     (8, 1500, 5128, 144), (8, 2000, 1704, 272), (16, 1280, 2696, 144), (24, 700, 2000, 656),
+                                     (8, 900, 1000, 1040), (2, 4500, 3000, 128), (300, 2400, 260, 256), (70, 20000, 256, 528)])
+def test_matmul_tile_sizes(gpu, E, R, N, K, dtype):
+    """Every tile, at its edges: sizes that fill the device, odd rows, columns and blocks; against 64 bits on
+    the device, the whole result."""
+    g = gen(R + N)
+    a, s = (t.to(gpu) for t in fp8_rows(g, R, K))
+    w, sw = (t.to(gpu) for t in fp8_weights(g, max(E, 1), N, K))
+    order = torch.randperm(R, generator=g).to(torch.int32)
+    order[R // 3] = -1
+    bounds = [0, R]
+    kw = {}
+    if E:
+        cut = torch.sort(torch.randint(0, R - 5, (E - 1,), generator=g)).values.tolist()
+        bounds = [3] + [max(3, c) for c in cut] + [R - 2]
+        kw["offsets"] = torch.tensor(bounds, dtype=torch.int32, device=gpu)
+    else:
+        w, sw = w[0], sw[0]
+    y = torch.full((R, N), 7.0, dtype=dtype, device=gpu)
+    qa.fp8_matmul(a, s, w, sw, rows=order.to(gpu), out=y, **kw)
+    assert (y[:bounds[0]] == 7).all() and (y[bounds[-1]:] == 7).all()
+    y = y.double()
+    at = order.long().to(gpu)
+    A = whole(a.float(), s)[at.clamp_min(0)] * (at >= 0)[:, None]
+    loss = (2 * 128 + blocks(K) + 8) * U32 + (7 * 2.0 ** -13 if dtype == torch.bfloat16 else 0)  # as check_product
+    for e in range(max(E, 1)):
+        i, j = bounds[e], bounds[e + 1]
+        if j > i:
+            W = whole((w[e] if E else w).float(), sw[e] if E else sw, 128)
+            want = A[i:j] @ W.T
+            size = A[i:j].abs() @ W.abs().T
+            off = (y[i:j] - want).abs() - loss * size * (1 + 2.0 ** -8) - U[dtype] * want.abs()
+            assert off.max() <= 0, f"expert {e}: {off.max().item():.3e} over its tolerance"
 
 
 @pytest.mark.gpu
@@ -472,7 +518,9 @@ def device_order(gpu, idx, E):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,E,k,kind", ORDERS + [(20000, 256, 8, "even"), (70001, 3, 2, "drop"), (30000, 1024, 4, "skew")])
+@pytest.mark.parametrize("T,E,k,kind", ORDERS + [(20000, 256, 8, "even"), (70001, 3, 2, "drop"), (30000, 1024, 4, "skew"),
+                                               (2000, 1024, 3, "drop"), (66000, 256, 8, "even"), (341, 64, 3, "drop"),
+                                               (342, 64, 3, "even")])
 def test_sort_tokens(gpu, T, E, k, kind):
     idx = routing(gen(T), T, E, k, kind)
     o = device_order(gpu, idx, E)
@@ -562,6 +610,39 @@ def test_token_gradients_against_differences(gpu):
         # p + d and p - d round once each, the sums of a forward k + 2 times, those of a gradient H + 8 times
         tol = (H + 2 * k + 16) * U32 * (size(up, f(hi)) + size(up, f(lo)) + size(grad, d) + size(grad, p)) * 4
         assert abs(slope - loss(grad, d)) <= tol
+
+
+@pytest.mark.gpu
+def test_token_outputs_given(gpu):
+    """Outputs in the caller's buffers, the sum into its residual; orders made by hand are checked."""
+    g = gen(6)
+    o = device_order(gpu, routing(g, 30, 8, 2), 8)
+    x, ys, w = randn(g, 30, 72).to(gpu), randn(g, 60, 72).to(gpu), torch.rand(30, 2, generator=g).to(gpu)
+    buf = torch.empty(60, 72, device=gpu)
+    assert qa.gather_tokens(x, o, out=buf) is buf and torch.equal(buf, qa.gather_tokens(x, o))
+    want = qa.combine_tokens(ys, o, w, residual=x)
+    res = x.clone()
+    assert qa.combine_tokens(ys, o, w, residual=res, out=res) is res and torch.equal(res, want)
+    back = torch.empty(30, 72, device=gpu)
+    assert qa.gather_tokens_backward(ys, o, out=back) is back
+    assert torch.equal(back, qa.combine_tokens(ys, o, torch.ones(30, 2, device=gpu)))
+    again = TokenOrder(o.offsets, o.rows, o.tokens, o.place)
+    assert torch.equal(qa.gather_tokens(x, again), buf) and again.n_experts == 8
+    for bad in ((o.offsets.long(), o.rows, o.tokens, o.place), (o.offsets[:1], o.rows, o.tokens, o.place),
+                (o.offsets, o.rows[:-1], o.tokens, o.place), (o.offsets, o.rows, o.tokens.cpu(), o.place),
+                (o.offsets, o.rows, o.tokens, o.place.t()), (o.offsets, o.rows, o.tokens, o.place.view(-1))):
+        with pytest.raises(ValueError, match="expected"):
+            TokenOrder(*bad)
+    with pytest.raises(ValueError, match="order expected"):
+        qa.gather_tokens(x, (o.offsets, o.place))
+    for out in (ys[:30], ys[7:37], ys[30:]):
+        with pytest.raises(qa.QmoeError, match="y expected a buffer distinct from ys, got an overlapping one"):
+            qa.combine_tokens(ys, o, w, out=out)
+    both = torch.zeros(40, 72, device=gpu)
+    with pytest.raises(qa.QmoeError, match="distinct from residual"):
+        qa.combine_tokens(ys, o, w, residual=both[:30], out=both[10:])
+    with pytest.raises(qa.QmoeError, match="distinct from x"):
+        qa.residual_norm(both[:30], both[10:], None, 1e-6, out=both[5:35])
 
 
 @pytest.mark.gpu
