@@ -11,7 +11,6 @@ namespace qmoe {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
@@ -30,7 +29,7 @@ __device__ __forceinline__ float fp8_act(int act, float g, float u) {
     return g / (1.0f + expf(-z)) * u;
 }
 
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_blocks, int cols, int act, uint8_t* q,
                                                       float* scale) {
     const uint32_t per_row = (uint32_t)(cols + kFp8Block - 1) / kFp8Block;
@@ -42,11 +41,11 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_
     float v[8] = {};
     if (n > 0) {
         if (act == kFp8ActNone) {
-            load8<BF16, VEC>(x, (uint64_t)row * cols + c0, n, v);
+            load8<BF16, WHOLE>(x, (uint64_t)row * cols + c0, n, v);
         } else {
             float u[8];
-            load8<BF16, VEC>(x, (uint64_t)row * 2 * cols + c0, n, v);
-            load8<BF16, VEC>(x, (uint64_t)row * 2 * cols + cols + c0, n, u);
+            load8<BF16, WHOLE>(x, (uint64_t)row * 2 * cols + c0, n, v);
+            load8<BF16, WHOLE>(x, (uint64_t)row * 2 * cols + cols + c0, n, u);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fp8_act(act, v[i], u[i]);
         }
@@ -55,16 +54,7 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_
     const float m = fp8_block_max(v, inv);
     uint32_t o[2];
     fp8_pack8(v, inv, o);
-    if (n > 0) {
-        uint8_t* qp = q + (uint64_t)row * cols + c0;
-        if (VEC) {
-            *(uint2*)qp = make_uint2(o[0], o[1]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < n) qp[i] = (uint8_t)(o[i >> 2] >> (8 * (i & 3)));
-        }
-    }
+    if (n > 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o);
     if ((threadIdx.x & 15) == 0) scale[id] = m / kFp8Max;
 }
 
@@ -73,11 +63,11 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
     const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
     if (blocks <= 0) return hipSuccess;
     if (blocks > 0xffffffffll) return hipErrorInvalidValue;
-    const bool vec = cols % 8 == 0 && (((uintptr_t)x | (uintptr_t)q) & 15u) == 0;
+    const bool whole = cols % 8 == 0;
     const dim3 grid((unsigned)((blocks + 15) / 16));
 #define QMOE_Q8(B, V) hipLaunchKernelGGL((k_fp8_quantize<B, V>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale)
-    if (bf16) { if (vec) QMOE_Q8(true, true); else QMOE_Q8(true, false); }
-    else { if (vec) QMOE_Q8(false, true); else QMOE_Q8(false, false); }
+    if (bf16) { if (whole) QMOE_Q8(true, true); else QMOE_Q8(true, false); }
+    else { if (whole) QMOE_Q8(false, true); else QMOE_Q8(false, false); }
 #undef QMOE_Q8
     return hipGetLastError();
 }
@@ -178,7 +168,8 @@ __device__ __forceinline__ int fp8_source_row(const Fp8Product& p, int r) {
     return s >= 0 && s < p.a_rows ? s : -1;
 }
 
-// C consecutive columns (4 or 8) of a row from column n on; those past N are left out.
+// C consecutive columns (4 or 8) of a row from column n on, up to 16 bytes at the elements'
+// alignment; those past N are left out.
 template <typename V>
 __device__ __forceinline__ void fp8_put(const Fp8Product& p, void* y, V v) {
     if (p.stream_out) {
@@ -193,14 +184,14 @@ template <bool BF16, int C>
 __device__ __forceinline__ void fp8_store(const Fp8Product& p, int r, int n, const float (&v)[C]) {
     static_assert(C == 4 || (C == 8 && BF16), "up to 16 bytes");
     const uint64_t at = (uint64_t)r * p.N + n;
-    if (p.vec_out && n + C <= p.N) {
+    if (n + C <= p.N) {
         if constexpr (!BF16) {
-            fp8_put(p, (float*)p.y + at, f32x4{v[0], v[1], v[2], v[3]});
+            fp8_put(p, (float*)p.y + at, f32x4a4{v[0], v[1], v[2], v[3]});
         } else if constexpr (C == 4) {
-            fp8_put(p, (uint16_t*)p.y + at, u32x2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3])});
+            fp8_put(p, (uint16_t*)p.y + at, u32x2a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3])});
         } else {
-            fp8_put(p, (uint16_t*)p.y + at, u32x4{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
-                                                  f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])});
+            fp8_put(p, (uint16_t*)p.y + at, u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
+                                                    f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])});
         }
     } else {
 #pragma unroll
@@ -601,7 +592,6 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     if (p.R <= 0) return hipSuccess;
     p.KB = (p.K + kFp8Block - 1) / kFp8Block;
     p.NB = (p.N + kFp8Block - 1) / kFp8Block;
-    p.vec_out = p.N % 8 == 0 && ((uintptr_t)p.y & 15u) == 0;
     // Workgroups of rows x cols tiles (grouped: at most).
     auto wgs = [&](int rows, int cols) { return fp8_max_tiles(p, rows) * ((p.N + cols - 1) / cols); };
     // A grid of at most two workgroups per CU that streams its operands once: latency.

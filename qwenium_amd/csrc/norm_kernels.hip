@@ -27,7 +27,7 @@ __device__ __forceinline__ double block_sum_f64(double v, double* s) {
     return t;
 }
 
-template <bool BF16, bool VEC, int NP>
+template <bool BF16, bool WHOLE, int NP>
 __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
     __shared__ double s_sum[2][16];
     const uint64_t row = (uint64_t)blockIdx.x * p.H;
@@ -39,9 +39,9 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
         c0[i] = 8 * ((int)threadIdx.x + i * (int)blockDim.x);
         n[i] = H - c0[i];  // columns from c0 on: none or some of the 8 may exist
         if (n[i] <= 0) continue;
-        load8<BF16, VEC>(p.x, row + c0[i], n[i], v[i]);
-        if (p.y) load8<BF16, VEC>(p.y, row + c0[i], n[i], u[i]);
-        if (p.gate) load8<BF16, VEC>(p.gate, row + c0[i], n[i], g[i]);
+        load8<BF16, WHOLE>(p.x, row + c0[i], n[i], v[i]);
+        if (p.y) load8<BF16, WHOLE>(p.y, row + c0[i], n[i], u[i]);
+        if (p.gate) load8<BF16, WHOLE>(p.gate, row + c0[i], n[i], g[i]);
     }
     if (p.y) {
         float post = 1.0f;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
             if (n[i] <= 0) continue;
             if (p.post_w) {
                 float w[8];
-                load8<false, VEC>(p.post_w, c0[i], n[i], w);
+                load8<false, WHOLE>(p.post_w, c0[i], n[i], w);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) u[i][c] = u[i][c] * post * w[c];
             }
@@ -71,14 +71,14 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
             }
             float sc[8];
             if (p.scale_v) {
-                load8<false, VEC>(p.scale_v, c0[i], n[i], sc);
+                load8<false, WHOLE>(p.scale_v, c0[i], n[i], sc);
             } else {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) sc[c] = p.scale;
             }
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[i][c] += sc[c] * u[i][c];
-            store8<BF16, VEC>(p.x_out, row + c0[i], n[i], v[i]);
+            store8<BF16, WHOLE>(p.x_out, row + c0[i], n[i], v[i]);
         }
     }
     double s = 0.0;
@@ -91,27 +91,21 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
     for (int i = 0; i < NP; ++i) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) w[i][c] = 1.0f;
-        if (p.w && n[i] > 0) load8<false, VEC>(p.w, c0[i], n[i], w[i]);
+        if (p.w && n[i] > 0) load8<false, WHOLE>(p.w, c0[i], n[i], w[i]);
     }
     const float r = rms_scale_from_ssq(block_sum_f64(s, s_sum[1]), H, p.eps);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) v[i][c] = v[i][c] * r * w[i][c];
-        if (n[i] > 0) store8<BF16, VEC>(p.h, row + c0[i], n[i], v[i]);
+        if (n[i] > 0) store8<BF16, WHOLE>(p.h, row + c0[i], n[i], v[i]);
         if (p.q) {
             float inv;
             const float m = fp8_block_max(v[i], inv);
             uint32_t o[2];
             fp8_pack8(v[i], inv, o);
             if (n[i] > 0) {
-                if (VEC) {
-                    *(uint2*)(p.q + row + c0[i]) = make_uint2(o[0], o[1]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        if (c < n[i]) p.q[row + c0[i] + c] = (uint8_t)(o[c >> 2] >> (8 * (c & 3)));
-                }
+                store8_fp8(p.q + row + c0[i], n[i], o);
                 const int nb = (H + kFp8Block - 1) / kFp8Block;
                 if ((threadIdx.x & 15) == 0) p.q_scale[(uint64_t)blockIdx.x * nb + c0[i] / kFp8Block] = m / kFp8Max;
             }
@@ -119,22 +113,20 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
     }
 }
 
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 static void launch_norm(const ResidualNorm& p, int n_tokens, hipStream_t stream) {
     const int pieces = (p.H + 7) / 8, np = pieces > 1024 ? 2 : 1;
     const dim3 grid(n_tokens), block((unsigned)(((pieces + np - 1) / np + 63) / 64 * 64));
-    if (np == 2) hipLaunchKernelGGL((k_residual_norm<BF16, VEC, 2>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((k_residual_norm<BF16, VEC, 1>), grid, block, 0, stream, p);
+    if (np == 2) hipLaunchKernelGGL((k_residual_norm<BF16, WHOLE, 2>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((k_residual_norm<BF16, WHOLE, 1>), grid, block, 0, stream, p);
 }
 
 hipError_t launch_residual_norm(const ResidualNorm& p, bool bf16, int n_tokens, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
     if (p.H > 16384) return hipErrorInvalidValue;
-    const uintptr_t any = (uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.gate | (uintptr_t)p.post_w | (uintptr_t)p.scale_v |
-                          (uintptr_t)p.w | (uintptr_t)p.x_out | (uintptr_t)p.h | (uintptr_t)p.q;
-    const bool vec = p.H % 8 == 0 && (any & 15u) == 0;
-    if (bf16) { if (vec) launch_norm<true, true>(p, n_tokens, stream); else launch_norm<true, false>(p, n_tokens, stream); }
-    else { if (vec) launch_norm<false, true>(p, n_tokens, stream); else launch_norm<false, false>(p, n_tokens, stream); }
+    const bool whole = p.H % 8 == 0;
+    if (bf16) { if (whole) launch_norm<true, true>(p, n_tokens, stream); else launch_norm<true, false>(p, n_tokens, stream); }
+    else { if (whole) launch_norm<false, true>(p, n_tokens, stream); else launch_norm<false, false>(p, n_tokens, stream); }
     return hipGetLastError();
 }
 

@@ -48,8 +48,13 @@ __device__ __forceinline__ uint32_t f32_pack_bf16(float lo, float hi) {
 }
 
 // Elements of a row of f32 or bf16, as f32: 8 from element `at` on, of which n exist
-// (the others 0, not stored).  VEC: all 8 exist and start 16-byte aligned.
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+// (the others 0, not stored).  WHOLE: all 8 exist.  16-byte accesses at the elements'
+// own alignment, so that rows of any width and start take them.
+typedef uint16_t u16x8a2 __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x2a1 __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 template <bool BF16>
 __device__ __forceinline__ float load1(const void* x, uint64_t at) {
     return BF16 ? bf16_to_f32(((const uint16_t*)x)[at]) : ((const float*)x)[at];
@@ -59,33 +64,47 @@ __device__ __forceinline__ void store1(void* y, uint64_t at, float v) {
     if (BF16) ((uint16_t*)y)[at] = (uint16_t)f32_pack_bf16(v, 0.0f);
     else ((float*)y)[at] = v;
 }
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 __device__ __forceinline__ void load8(const void* x, uint64_t at, int n, float (&v)[8]) {
-    if constexpr (VEC && BF16) {
-        const u16x8 r = *(const u16x8*)((const uint16_t*)x + at);
+    if (WHOLE || n >= 8) {
+        if constexpr (BF16) {
+            const u16x8a2 r = *(const u16x8a2*)((const uint16_t*)x + at);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(r[i]);
-    } else if constexpr (VEC) {
-        const f32x4 r = *(const f32x4*)((const float*)x + at), s = *(const f32x4*)((const float*)x + at + 4);
+            for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(r[i]);
+        } else {
+            const f32x4a4 r = *(const f32x4a4*)((const float*)x + at), s = *(const f32x4a4*)((const float*)x + at + 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = r[i], v[4 + i] = s[i];
+            for (int i = 0; i < 4; ++i) v[i] = r[i], v[4 + i] = s[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < n ? load1<BF16>(x, at + i) : 0.0f;
     }
 }
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 __device__ __forceinline__ void store8(void* y, uint64_t at, int n, const float (&v)[8]) {
-    if constexpr (VEC && BF16) {
-        *(u32x4*)((uint16_t*)y + at) = u32x4{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
-                                             f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])};
-    } else if constexpr (VEC) {
-        *(f32x4*)((float*)y + at) = f32x4{v[0], v[1], v[2], v[3]};
-        *(f32x4*)((float*)y + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    if (WHOLE || n >= 8) {
+        if constexpr (BF16) {
+            *(u32x4a2*)((uint16_t*)y + at) = u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
+                                                     f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])};
+        } else {
+            *(f32x4a4*)((float*)y + at) = f32x4a4{v[0], v[1], v[2], v[3]};
+            *(f32x4a4*)((float*)y + at + 4) = f32x4a4{v[4], v[5], v[6], v[7]};
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < n) store1<BF16>(y, at + i, v[i]);
+    }
+}
+// 8 packed e4m3 values, of which n exist.
+__device__ __forceinline__ void store8_fp8(uint8_t* q, int n, const uint32_t (&o)[2]) {
+    if (n >= 8) {
+        *(u32x2a1*)q = u32x2a1{o[0], o[1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) q[i] = (uint8_t)(o[i >> 2] >> (8 * (i & 3)));
     }
 }
 

@@ -60,8 +60,7 @@ struct Fp8Product {
     const int32_t* rows;
     void* y;
     int a_rows, E, N, K, R;
-    int KB, NB;     // blocks of 128 along K and N (set by the launcher)
-    bool vec_out;     // y's rows take aligned stores of 16 bytes (set by the launcher)
+    int KB, NB;       // blocks of 128 along K and N (set by the launcher)
     bool stream_out;  // y past the caches (set by the launcher)
 };
 

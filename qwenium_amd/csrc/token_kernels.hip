@@ -192,45 +192,44 @@ static void row_grid(int n_tokens, int64_t pieces, dim3& grid, dim3& block) {
 // Rows to the experts' order: a token's workgroups read its row once and write it
 // top_k times (reading by sorted row would read it top_k times).  Rows behind the
 // last expert's belong to no token: zeros, by the token with those list indices.
-// Pieces of 16 bytes (V = u32x4) or single elements.
+// A thread takes 16 bytes; a row's last 16 may overlap the ones before (the same
+// bytes written twice).  V: 16 bytes, or single bytes for rows shorter than that.
 // ---------------------------------------------------------------------------
+typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));
 template <typename V>
-__global__ __launch_bounds__(256) void k_gather_tokens(const V* x, int n, int top_k, int R, const int32_t* total,
-                                                       const int32_t* place, V* y) {
-    const int t = blockIdx.x, i = blockIdx.y * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    const V v = x[(uint64_t)t * n + i];
+__global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int bytes, int top_k, int R, const int32_t* total,
+                                                       const int32_t* place, uint8_t* y) {
+    constexpr int kSize = sizeof(V);
+    const int t = blockIdx.x;
+    int i = kSize * (int)(blockIdx.y * blockDim.x + threadIdx.x);
+    if (i >= bytes) return;
+    if (i + kSize > bytes) i = bytes - kSize;
+    const V v = *(const V*)(x + (uint64_t)t * bytes + i);
     const int32_t* pl = place + (int64_t)t * top_k;
     const int last = *total;
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
         const int p = pl[j];
-        if (p >= 0 && p < R) y[(uint64_t)p * n + i] = v;
+        if (p >= 0 && p < R) *(V*)(y + (uint64_t)p * bytes + i) = v;
         const int r = t * top_k + j;
-        if (r >= last) y[(uint64_t)r * n + i] = V{};
+        if (r >= last) *(V*)(y + (uint64_t)r * bytes + i) = V{};
     }
-}
-
-template <typename V>
-static hipError_t launch_gather(const void* x, int64_t n, int n_tokens, int top_k, const int32_t* total, const int32_t* place,
-                                void* y, hipStream_t stream) {
-    dim3 grid, block;
-    row_grid(n_tokens, n, grid, block);
-    if (grid.y > 65535) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_gather_tokens<V>, grid, block, 0, stream, (const V*)x, (int)n, top_k, n_tokens * top_k, total, place,
-                       (V*)y);
-    return hipGetLastError();
 }
 
 hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_cols, int top_k, const int32_t* total,
                                 const int32_t* place, void* y, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const int64_t bytes = (int64_t)n_cols * elem;
-    if (bytes % 16 == 0 && (((uintptr_t)x | (uintptr_t)y) & 15u) == 0)
-        return launch_gather<u32x4>(x, bytes / 16, n_tokens, top_k, total, place, y, stream);
-    if (elem == 4) return launch_gather<uint32_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
-    if (elem == 2) return launch_gather<uint16_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
-    return launch_gather<uint8_t>(x, n_cols, n_tokens, top_k, total, place, y, stream);
+    const int bytes = n_cols * elem;
+    dim3 grid, block;
+    row_grid(n_tokens, bytes >= 16 ? (bytes + 15) / 16 : bytes, grid, block);
+    if (grid.y > 65535) return hipErrorInvalidValue;
+    if (bytes >= 16)
+        hipLaunchKernelGGL(k_gather_tokens<u32x4a1>, grid, block, 0, stream, (const uint8_t*)x, bytes, top_k, n_tokens * top_k,
+                           total, place, (uint8_t*)y);
+    else
+        hipLaunchKernelGGL(k_gather_tokens<uint8_t>, grid, block, 0, stream, (const uint8_t*)x, bytes, top_k, n_tokens * top_k,
+                           total, place, (uint8_t*)y);
+    return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -238,13 +237,13 @@ hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_col
 // once (w null: ones, the gather's gradient).  Assignments without a place add
 // nothing.  8 columns a thread, the rows of 8 assignments in flight.
 // ---------------------------------------------------------------------------
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, int top_k, int R, const int32_t* place,
                                                         const float* w, const void* residual, void* y) {
     const int t = blockIdx.x, c0 = 8 * (blockIdx.y * blockDim.x + threadIdx.x), n = H - c0;
     if (n <= 0) return;
     float s[8] = {}, res[8] = {};
-    if (residual) load8<BF16, VEC>(residual, (uint64_t)t * H + c0, n, res);
+    if (residual) load8<BF16, WHOLE>(residual, (uint64_t)t * H + c0, n, res);
     for (int j0 = 0; j0 < top_k; j0 += 8) {
         float v[8][8], wj[8];
         bool has[8];
@@ -254,7 +253,7 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, i
             const int p = place[a];
             has[j] = j0 + j < top_k && p >= 0 && p < R;
             wj[j] = w ? w[a] : 1.0f;
-            if (has[j]) load8<BF16, VEC>(ys, (uint64_t)p * H + c0, n, v[j]);
+            if (has[j]) load8<BF16, WHOLE>(ys, (uint64_t)p * H + c0, n, v[j]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -264,20 +263,20 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, i
     }
 #pragma unroll
     for (int c = 0; c < 8; ++c) s[c] += res[c];
-    store8<BF16, VEC>(y, (uint64_t)t * H + c0, n, s);
+    store8<BF16, WHOLE>(y, (uint64_t)t * H + c0, n, s);
 }
 
 hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H, int top_k, const int32_t* place,
                                  const float* w, const void* residual, void* y, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const bool vec = H % 8 == 0 && (((uintptr_t)ys | (uintptr_t)residual | (uintptr_t)y) & 15u) == 0;
+    const bool whole = H % 8 == 0;
     dim3 grid, block;
     row_grid(n_tokens, ((int64_t)H + 7) / 8, grid, block);
     if (grid.y > 65535) return hipErrorInvalidValue;
 #define QMOE_COMBINE(B, V) \
     hipLaunchKernelGGL((k_combine_tokens<B, V>), grid, block, 0, stream, ys, H, top_k, n_tokens * top_k, place, w, residual, y)
-    if (bf16) { if (vec) QMOE_COMBINE(true, true); else QMOE_COMBINE(true, false); }
-    else { if (vec) QMOE_COMBINE(false, true); else QMOE_COMBINE(false, false); }
+    if (bf16) { if (whole) QMOE_COMBINE(true, true); else QMOE_COMBINE(true, false); }
+    else { if (whole) QMOE_COMBINE(false, true); else QMOE_COMBINE(false, false); }
 #undef QMOE_COMBINE
     return hipGetLastError();
 }
@@ -289,7 +288,7 @@ hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H,
 // columns and 8 assignments in flight), then the tree over its wave's lanes and
 // the waves in turn.  Rows behind the last expert's get zeros.
 // ---------------------------------------------------------------------------
-template <bool BF16, bool VEC>
+template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
                                                              const int32_t* total, const int32_t* place, const float* w,
                                                              void* dys, float* dw) {
@@ -301,11 +300,11 @@ __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, con
         for (int c0 = 8 * threadIdx.x; c0 < H; c0 += 8 * blockDim.x) {
             const int n = H - c0;
             float g[8], v[8][8];
-            load8<BF16, VEC>(dy, (uint64_t)t * H + c0, n, g);
+            load8<BF16, WHOLE>(dy, (uint64_t)t * H + c0, n, g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int p = j0 + j < top_k ? place[t * top_k + j0 + j] : -1;
-                if (p >= 0 && p < R) load8<BF16, VEC>(ys, (uint64_t)p * H + c0, n, v[j]);
+                if (p >= 0 && p < R) load8<BF16, WHOLE>(ys, (uint64_t)p * H + c0, n, v[j]);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -319,12 +318,12 @@ __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, con
                         dot[j] = fmaf(g[c], v[j][c], dot[j]);
                         o[c] = wj * g[c];
                     }
-                    store8<BF16, VEC>(dys, (uint64_t)p * H + c0, n, o);
+                    store8<BF16, WHOLE>(dys, (uint64_t)p * H + c0, n, o);
                 }
                 if (a >= last) {
 #pragma unroll
                     for (int c = 0; c < 8; ++c) o[c] = 0.0f;
-                    store8<BF16, VEC>(dys, (uint64_t)a * H + c0, n, o);
+                    store8<BF16, WHOLE>(dys, (uint64_t)a * H + c0, n, o);
                 }
             }
         }
@@ -348,14 +347,14 @@ hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, 
                                      const int32_t* total, const int32_t* place, const float* w, void* dys, float* dw,
                                      hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const bool vec = H % 8 == 0 && (((uintptr_t)dy | (uintptr_t)ys | (uintptr_t)dys) & 15u) == 0;
+    const bool whole = H % 8 == 0;
     const int64_t pieces = ((int64_t)H + 7) / 8;
     const dim3 grid(n_tokens), block((unsigned)(pieces < 1024 ? (pieces + 63) / 64 * 64 : 1024));
 #define QMOE_BWD(B, V)                                                                                                \
     hipLaunchKernelGGL((k_combine_tokens_bwd<B, V>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, place, w, \
                        dys, dw)
-    if (bf16) { if (vec) QMOE_BWD(true, true); else QMOE_BWD(true, false); }
-    else { if (vec) QMOE_BWD(false, true); else QMOE_BWD(false, false); }
+    if (bf16) { if (whole) QMOE_BWD(true, true); else QMOE_BWD(true, false); }
+    else { if (whole) QMOE_BWD(false, true); else QMOE_BWD(false, false); }
 #undef QMOE_BWD
     return hipGetLastError();
 }
