@@ -95,7 +95,7 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // 99 at the 2.8 PFLOP/s of a library e4m3 product without block scales; 111 without the
 // loads of the loop, 103 without its barriers too), f32 229 (1.2, as a library bf16
 // product); 256 experts of 1024 x 2048: 80 rows 29 (147 MB: 5.0 TB/s), 4096 rows 85
-// (6.3 TB/s), 32768 rows 142 (613 MB: 4.3 TB/s).
+// (6.3 TB/s), 32768 rows 138-142 (613 MB: 4.3-4.4 TB/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -607,16 +607,17 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
     }
     // By the rows an expert has on average: the tile that holds most experts' rows with few rows to
-    // spare.  256 experts of 1024 x 2048, bf16, us with 256x256 / 160x128 / 128x256 / 64x128: 32 rows
-    // 123 / 107 / 104 / 99, 64 rows 133 / 121 / 114 / 125, 128 rows 153 / 158 / 154 / 194, 187 rows
-    // 182 / 210 / 204 / 259; 128 experts of 2816 x 704: 125 rows 109 / 99 / 109 / 118; f32, 128 rows
-    // 240 / 206 / 222 / 241 (all with weights and results through the caches).
-    const int64_t mean = p.R / p.E, most = mean + mean / 7;  // (most experts' rows, evenly drawn)
+    // spare.  256 experts of 1024 x 2048, us with 256x256 / 160x128 / 128x256 / 64x128, bf16: 32 rows
+    // 123 / 107 / 104 / 99 and 64 rows 133 / 121 / 114 / 125 (all through the caches), 93 rows
+    // 130 / 122 / 111, 128 rows 150 / 138 / 151, 156 rows 162 / 166 / 185, 187 rows 177 / 209 / 202; f32:
+    // 93 rows 165 / 180 / 166, 128 rows 219 / 196 / 218, 156 rows 261 / 235 / 261, 187 rows 266 / 300 /
+    // 306; 64 experts of 1536 x 1536: 281 rows 87 / 79 / 90, f32 147 / 116 / 134.
+    const int64_t mean = p.R / p.E;
     // bf16 results larger than an L2 past the caches where the weights go past them: 32768 rows 150 / 142 us,
     // 4096 rows (8 MB) 89 / 85, the quantization after them no slower; 512 rows (1 MB) 69 / 72; f32 197 / 201.
-    p.stream_out = bf16 && most <= 256 && (int64_t)p.R * p.N * 2 > (4 << 20);
+    p.stream_out = bf16 && mean <= 256 && (int64_t)p.R * p.N * 2 > (4 << 20);
     if (mean >= 110) {
-        if ((most + 255) / 256 * 256 < (most + 159) / 160 * 160 && wgs(256, 256) >= kFp8Cus)
+        if (((mean > 160 && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
             return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
     } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
