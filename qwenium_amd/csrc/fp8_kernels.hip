@@ -16,17 +16,26 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------
 // Quantization.  Block b of a row: m = max(|v|, kFp8Tiny) over its 128 columns
 // (NaN counts as the largest, so a block with a NaN has a NaN scale),
-//   scale = m / 448,  q = e4m3(f32(v * f32(448 / m))), nearest, ties to even.
-// 448 is e4m3's largest value: the products stay within 448 (1 + 2^-22), which
-// rounds to it.  kFp8Tiny keeps 448 / m finite; a block of zeros has zeros.
+//   scale = m / 448,  q = e4m3(v * 448 / m), nearest, ties to even.
+// 448 is e4m3's largest value.  kFp8Tiny keeps 448 / m finite; a block of zeros has
+// zeros.
 // 16 lanes take a block, 8 columns each (one or two 16-byte loads), so a wave
-// covers 512 columns; no LDS, no barrier.
+// covers 512 columns; no LDS, no barrier.  Bound by memory: 4096 x 2048 f32 (42 MB) 8.2
+// us, 5.1 TB/s (0.5 of it for the exact quotients); 32768 x 512 SwiGLU of bf16 (84 MB)
+// 19.9 us, 4.2 TB/s, level with its arithmetic (21.0 with a division per value).
 // ---------------------------------------------------------------------------
+// g sigmoid(z) u.  Every rounding takes some values that lie next to an e4m3 border to its
+// other side: 1 / (1 + e) is an approximate reciprocal, whose remainder (with what 1 + e
+// dropped) corrects the quotient within the product with u.
 __device__ __forceinline__ float fp8_act(int act, float g, float u) {
     if (act == kFp8ActNone) return g;
     // gelu's tanh form is g sigmoid(2 z) with z = sqrt(2/pi) (g + 0.044715 g^3)
-    const float z = act == kFp8ActSwiglu ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-    return g / (1.0f + expf(-z)) * u;
+    const float z = act == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+    const float e = expf(-z), d = 1.0f + e;
+    if (!(d < 1e30f)) return g / d * u;  // (and NaN)
+    const float low = e > 1.0f ? 1.0f - (d - e) : e - (d - 1.0f);
+    const float r = __builtin_amdgcn_rcpf(d), q = g * r;
+    return fmaf(q, u, fmaf(-q, low, fmaf(-q, d, g)) * r * u);
 }
 
 template <bool BF16, bool WHOLE>
@@ -50,10 +59,9 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_
             for (int i = 0; i < 8; ++i) v[i] = fp8_act(act, v[i], u[i]);
         }
     }
-    float inv;
-    const float m = fp8_block_max(v, inv);
+    const float m = fp8_block_max(v);
     uint32_t o[2];
-    fp8_pack8(v, inv, o);
+    fp8_pack8(v, m, o);
     if (n > 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o);
     if ((threadIdx.x & 15) == 0) scale[id] = m / kFp8Max;
 }

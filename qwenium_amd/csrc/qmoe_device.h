@@ -111,9 +111,9 @@ __device__ __forceinline__ void store8_fp8(uint8_t* q, int n, const uint32_t (&o
 // ---------------------------------------------------------------------------
 // e4m3 blocks of 128 values, 8 per lane of 16 lanes.
 // ---------------------------------------------------------------------------
-// The block's largest |v| (at least kFp8Tiny) in all 16 lanes, and f32(448 / it).  The
-// bits of |v| order as integers, a NaN above infinity: it wins.
-__device__ __forceinline__ float fp8_block_max(const float (&v)[8], float& inv) {
+// The block's largest |v| (at least kFp8Tiny) in all 16 lanes.  The bits of |v| order as
+// integers, a NaN above infinity: it wins.
+__device__ __forceinline__ float fp8_block_max(const float (&v)[8]) {
     uint32_t m = __builtin_bit_cast(uint32_t, kFp8Tiny);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -125,16 +125,41 @@ __device__ __forceinline__ float fp8_block_max(const float (&v)[8], float& inv) 
         const uint32_t b = (uint32_t)__shfl_xor((int)m, o, 64);
         m = b > m ? b : m;
     }
-    const float top = __builtin_bit_cast(float, m);
-    inv = kFp8Max / top;
-    return top;
+    return __builtin_bit_cast(float, m);
 }
-__device__ __forceinline__ void fp8_pack8(const float (&v)[8], float inv, uint32_t (&o)[2]) {
+// A value that rounds to e4m3 as the exact v * 448 / m does (ties to even): p = v * f32(448 /
+// m) is within two of its last places of that, and next to e4m3's border t (the middle of
+// two neighbours) the side is decided by |v| 448 against t m, both exact in f64.
+__device__ __forceinline__ float fp8_quotient(float v, float inv, float m) {
+    const float p = v * inv;
+    const uint32_t b = __builtin_bit_cast(uint32_t, p), a = b & 0x7fffffffu;
+    const bool small = a < 0x3c800000u;  // |p| < 2^-6: steps of 2^-9
+    if (a == 0 || (!small && ((b - 0x7fffeu) & 0xfffffu) > 4u)) return p;
+    const float t = small ? (floorf(__builtin_fabsf(p) * 512.0f) + 0.5f) * (1.0f / 512.0f)
+                          : __builtin_bit_cast(float, (a & 0xfff00000u) | 0x80000u);
+    const double d = (double)__builtin_fabsf(v) * 448.0 - (double)t * (double)m;
+    const uint32_t r = __builtin_bit_cast(uint32_t, t) + (d > 0.0 ? 1u : d < 0.0 ? ~0u : 0u);
+    return __builtin_bit_cast(float, r | (b & 0x80000000u));
+}
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
+// e4m3 of the exact v * 448 / m, rounded once.  Quotients a little (2^-22 of them) above and
+// below mostly round to the same numbers, and then the exact ones do.
+__device__ __forceinline__ void fp8_pack8(const float (&v)[8], float m, uint32_t (&o)[2]) {
+    const float inv = kFp8Max / m, up = inv * (1.0f + 0x1p-22f), down = inv * (1.0f - 0x1p-22f);
+    uint32_t other = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * inv, v[4 * h + 1] * inv, 0, false);
-        o[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * inv, v[4 * h + 3] * inv, r, true);
+        const float* x = v + 4 * h;
+        o[h] = fp8_pack4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
+        other |= o[h] ^ fp8_pack4(x[0] * down, x[1] * down, x[2] * down, x[3] * down);
     }
+    if (other == 0) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        o[h] = fp8_pack4(fp8_quotient(h ? v[4] : v[0], inv, m), fp8_quotient(h ? v[5] : v[1], inv, m),
+                         fp8_quotient(h ? v[6] : v[2], inv, m), fp8_quotient(h ? v[7] : v[3], inv, m));
 }
 
 // ---------------------------------------------------------------------------
