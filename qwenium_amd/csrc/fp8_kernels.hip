@@ -383,8 +383,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     static_assert(T::slot_w(8 * T::kWaves) == 0, "the same slots in every group of a wave");
     // (a tile whose row groups do not divide among the waves: the last ones load some again)
     auto group_a = [&](int i) {
-        const int g = wave + T::kWaves * i;
-        return T::kBM / 8 % T::kWaves == 0 || g < T::kBM / 8 ? g : g - T::kWaves;
+        return (wave + T::kWaves * i) % (T::kBM / 8);
     };
     const uint8_t* ga[kGA];
 #pragma unroll
@@ -544,9 +543,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
             for (int l = 0; l < T::kLoads; ++l) load(l, b, b);
     const int subs = (nrows + 15) >> 4;                     // subtiles with rows
     const int mine = subs > wm ? (subs - wm + WM - 1) / WM : 0;  // ... of this wave
-    if (mine > MS / 2) run(std::integral_constant<int, MS>{});
-    else if (mine > MS / 4) run(std::integral_constant<int, MS / 2>{});
-    else run(std::integral_constant<int, MS / 4>{});
+    constexpr int kHalf = MS / 2 > 1 ? MS / 2 : 1, kQuarter = MS / 4 > 1 ? MS / 4 : 1;
+    if (mine > kHalf) run(std::integral_constant<int, MS>{});
+    else if (mine > kQuarter) run(std::integral_constant<int, kHalf>{});
+    else run(std::integral_constant<int, kQuarter>{});
 
 #pragma unroll
     for (int i = 0; i < MS; ++i) {
@@ -631,7 +631,14 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
         return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
     }
-    if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
+    // Weights streamed for few rows: small tiles, many loads in flight, unless K is soon over.  Four layers'
+    // weights in turn, us with 32x64 in four buffers / 64x128 in three / in two: 256 experts of 1024 x 2048, 2
+    // tokens 8.4 / 11.2 / 17.1, 10 tokens 25 / 28 / 25, 64 69 / 71 / 76, 512 89 / 90 / 93; 32 of 2048 x 4096,
+    // 100 tokens 51 / 59 / 61; 128 of 2816 x 704, 64 tokens 54 / 54 / 53; 256 of 2048 x 512, 64 tokens 45 / 43 /
+    // 40, 211 tokens 52 / 51 / 49.
+    if (mean < 20 && p.KB >= 8) return launch_tile<1, 4, 2, 1, 4>(p, bf16, stream);
+    if (wgs(64, 128) >= kFp8Cus)
+        return p.KB <= 4 ? launch_tile<1, 4, 4, 2, 2>(p, bf16, stream) : launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
     return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
 }
 
