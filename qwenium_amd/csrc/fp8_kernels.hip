@@ -99,11 +99,11 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // stores them together.  (Both operands take the same permutation of a block's
 // columns, which leaves its sum as it is: lane group g reads 16-byte pieces g and
 // g + 4.)
-//   Where the time goes (us): 8192 x 4096 x 4096 bf16 131 (2.1 PFLOP/s; 275 GFLOP take
+//   Where the time goes (us): 8192 x 4096 x 4096 bf16 132 (2.1 PFLOP/s; 275 GFLOP take
 // 99 at the 2.8 PFLOP/s of a library e4m3 product without block scales; 111 without the
 // loads of the loop, 103 without its barriers too), f32 229 (1.2, as a library bf16
-// product); 256 experts of 1024 x 2048: 80 rows 29 (147 MB: 5.0 TB/s), 4096 rows 85
-// (6.3 TB/s), 32768 rows 138-142 (613 MB: 4.3-4.4 TB/s).
+// product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
+// (6.3 TB/s), 32768 rows 139-142 (613 MB: 4.3-4.4 TB/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -317,11 +317,6 @@ __global__ __launch_bounds__(256) void k_fp8_stream(Fp8Product p) {
     }
 }
 
-// Many rows: a workgroup of WM x WN waves makes a tile of 16 MS WM rows and 16 NS WN
-// columns.  Each step of 128 columns of K comes straight to LDS (two buffers, one
-// step ahead): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
-// (row & 7), so that the 16 rows of a fragment meet all banks.  The 16-row subtiles
-// go to the WM waves in turn and those without rows are left out (MI: how many).
 // A wave-uniform read-only value through the scalar cache: no vector memory load, whose
 // wait would be one for all direct loads before it.
 __device__ __forceinline__ float scalar_load(const float* p) {
@@ -356,6 +351,12 @@ struct Fp8Tile {
     static_assert(16 * NS <= kFp8Block, "a wave's columns share one scale");
 };
 
+// Many rows: a workgroup of WM x WN waves makes a tile of 16 MS WM rows and 16 NS WN
+// columns.  Each step of 128 columns of K comes straight to LDS (ST buffers, ST - 1
+// steps ahead): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
+// (row & 7), so that the 16 rows of a fragment meet all banks (measured: no conflicts).
+// The 16-row subtiles go to the WM waves in turn and those without rows are left out
+// (MI: how many).
 template <int WM, int WN, int MS, int NS, int ST, bool BF16>
 __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
