@@ -99,10 +99,10 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // stores them together.  (Both operands take the same permutation of a block's
 // columns, which leaves its sum as it is: lane group g reads 16-byte pieces g and
 // g + 4.)
-//   Where the time goes (us): 8192 x 4096 x 4096 bf16 132 (2.1 PFLOP/s; 275 GFLOP take
-// 99 at the 2.8 PFLOP/s of a library e4m3 product without block scales; 111 without the
-// loads of the loop, 103 without its barriers too), f32 229 (1.2, as a library bf16
-// product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
+//   Where the time goes (us): 8192 x 4096 x 4096 bf16 128 (2.1 PFLOP/s; 275 GFLOP take
+// 93-104 in a library e4m3 product without block scales): the matrix instructions alone
+// 73, with the fmas of the scales 94, with the reads of LDS 103, the rest the loads to
+// it, 10 of that past the L2; f32 228 (1.2, as a library bf16 product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
 // (6.3 TB/s), 32768 rows 139-142 (613 MB: 4.3-4.4 TB/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -352,8 +352,7 @@ struct Fp8Tile {
 };
 
 // Many rows: a workgroup of WM x WN waves makes a tile of 16 MS WM rows and 16 NS WN
-// columns.  Each step of 128 columns of K comes straight to LDS (ST buffers, ST - 1
-// steps ahead): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
+// columns.  Each step of 128 columns of K comes straight to LDS (ST buffers): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
 // (row & 7), so that the 16 rows of a fragment meet all banks (measured: no conflicts).
 // The 16-row subtiles go to the WM waves in turn and those without rows are left out
 // (MI: how many).
@@ -408,32 +407,41 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
         gs = p.sa + (uint64_t)(s < 0 ? 0 : s) * KB;
         s_none[r] = s < 0;
     }
-    // load l of step b into buffer buf: the rows' groups, the weights', the row scales
-    const uint32_t lds0 = lds_addr(s_dyn);
-    auto load = [&](int l, int b, int buf) {
-        const int c = b * kFp8Block + (l < kGA ? piece : piece_w);
-        const int at = c < p.K ? c : p.K - 16;  // past K: any valid piece, its weights are zeroed below
-        const uint32_t base = lds0 + buf * T::kStage;
-        if (l < kGA) dma_lds16_at(ga[l] + at, base + 1024 * group_a(l));
-        else {
-            const uint32_t to = base + T::kBM * kFp8Block + 1024 * (wave + T::kWaves * (l - kGA));
-            if (once) dma_lds16<true>(wt, gw[l - kGA] + (uint32_t)at, to);
-            else dma_lds16<false>(wt, gw[l - kGA] + (uint32_t)at, to);
-        }
-    };
     // The row scales of steps b .. b + 3, by the waves 0 .. kScaleLoads - 1: 64 rows each, 16 bytes a row
     // (a row's scales lie KB apart: one 64-row load of single scales costs as much).  Where KB is no
     // multiple of 4, four loads of one step each.
     const bool quads = KB % 4 == 0 && ((uintptr_t)p.sa & 15) == 0;
     auto load_scales = [&](int b) {
         if (wave >= T::kScaleLoads) return;
-        const uint32_t base = lds0 + ST * T::kStage + (b >> 2 & 1) * T::kScales + 1024 * wave;
+        const uint32_t base = lds_addr(s_dyn) + ST * T::kStage + (b >> 2 & 1) * T::kScales + 1024 * wave;
         if (quads) {
             dma_lds16_at(gs + b, base);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) dma_lds4_at(gs + (b + i < KB ? b + i : KB - 1), base + 256 * i);
         }
+    };
+    // This wave's loads [from, to) of step b into buffer buf, of kLoads: the rows' groups (the row scales of four steps
+    // first), then the weights'.
+    const uint32_t lds0 = lds_addr(s_dyn);
+    auto load = [&](int b, int buf, int from, int to) {
+        if (from == 0 && b % 4 == 0) load_scales(b);
+        // past K: any valid piece, its weights are zeroed below
+        auto column = [&](int piece) { const int c = b * kFp8Block + piece; return c < p.K ? c : p.K - 16; };
+        const uint32_t base = lds0 + buf * T::kStage;
+        const int ca = column(piece), cw = column(piece_w);
+#pragma unroll
+        for (int i = 0; i < kGA; ++i)
+            if (i >= from && i < to) dma_lds16_at(ga[i] + ca, base + 1024 * group_a(i));
+        auto weights = [&](auto nt_c) {
+#pragma unroll
+            for (int i = 0; i < kGW; ++i)
+                if (kGA + i >= from && kGA + i < to)
+                    dma_lds16<decltype(nt_c)::value>(wt, gw[i] + (uint32_t)cw,
+                                                     base + T::kBM * kFp8Block + 1024 * (wave + T::kWaves * i));
+        };
+        if (once) weights(std::true_type{});
+        else weights(std::false_type{});
     };
     const int scale_row = quads ? 16 : 4, scale_step = quads ? 4 : 256;  // LDS distances
 
@@ -444,104 +452,136 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     const int fw = T::kCols * (fr >> 2) + (fr & 3);  // this lane's weight row of subtile 0
     const int wpiece0 = fw * kFp8Block + 16 * (fg ^ T::slot_w(fw)), wpiece1 = wpiece0 ^ 64;
     f32x4 acc[MS][NS] = {};
+    // A step's weight fragments, and its first row fragment, are read while the step before it makes its last products.
     auto run = [&](auto mi_c) {
         constexpr int MI = decltype(mi_c)::value;
-        int buf = 0, next = ST - 1;
+        constexpr int kLate = MI >= 4 ? 2 : 1;  // subtiles whose products come after the step's last row fragment is read
+        // Eight waves load half of a stage after the barrier, half in the next step: all at once they hold each other up
+        // (8192 x 4096 x 4096 bf16 134 us, in halves 128; tiles of four waves lose 1-2% by it).
+        constexpr int kFirst = T::kWaves == 8 && MI >= 4 ? (T::kLoads + 1) / 2 : T::kLoads;
+        int buf = 0;
         float ws_next = scalar_load(sw);
-        // TAIL: step b is the last and shorter than a block
-        auto step = [&](int b, auto tail_c) {
-            constexpr bool TAIL = decltype(tail_c)::value;
-            // step b has landed (at most the ST - 2 after it are in flight) ...
-            // (a wave's scale loads come before its stage's: they have landed with it)
-            if (!TAIL && b + ST - 2 < KB) __builtin_amdgcn_s_waitcnt(vm_wait((ST - 2) * T::kLoads));
-            else __builtin_amdgcn_s_waitcnt(vm_wait(0));
-            lds_barrier();  // ... for every wave, and the oldest buffer is no longer read
+        i32x8 av[3], wv[NS];  // (whole operands: halves carried apart would be copied together)
+        float rs[3];
+        auto join = [](i32x4 lo, i32x4 hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); };
+        // subtile 0 has fragment registers of its own
+        auto slot = [](int i) { return i == 0 ? 2 : (i - 1) & 1; };
+        auto rows = [&](int i, int b, int at) {
+            const uint8_t* st = s_dyn + at * T::kStage;
+            const uint8_t* scales = s_dyn + ST * T::kStage + (b >> 2 & 1) * T::kScales + (b & 3) * scale_step + fr * scale_row;
+            const int sub = WM * i + wm, x = slot(i);
+            av[x] = join(*(const i32x4*)(st + 16 * sub * kFp8Block + piece0), *(const i32x4*)(st + 16 * sub * kFp8Block + piece1));
+            // (subtile sub is rows 16 (sub % 4) .. of load sub / 4)
+            rs[x] = *(const float*)(scales + 1024 * (sub >> 2) + 16 * (sub & 3) * scale_row);
+        };
+        auto weights = [&](int n, int at) {
+            const uint8_t* w = s_dyn + at * T::kStage +
+                               (T::kBM + 16 * NS * wn + 4 * T::kCols * (n / T::P) + 4 * (n % T::P)) * kFp8Block;
+            wv[n] = join(*(const i32x4*)(w + wpiece0), *(const i32x4*)(w + wpiece1));
+        };
+        // LAST: no step follows, and K may end inside its block
+        auto step = [&](int b, auto last_c) {
+            constexpr bool LAST = decltype(last_c)::value;
             const float ws = ws_next;
             ws_next = scalar_load(sw + (b + 1 < KB ? b + 1 : b));
-            const uint8_t* st = s_dyn + buf * T::kStage;
-            const uint8_t* scales = s_dyn + ST * T::kStage + (b >> 2 & 1) * T::kScales + (b & 3) * scale_step + fr * scale_row;
-            i32x4 al[2], ah[2], wl[NS], wh[NS];
-            float rs[2];
-            auto rows = [&](int i) {
-                const int sub = WM * i + wm;
-                al[i & 1] = *(const i32x4*)(st + 16 * sub * kFp8Block + piece0);
-                ah[i & 1] = *(const i32x4*)(st + 16 * sub * kFp8Block + piece1);
-                // (subtile sub is rows 16 (sub % 4) .. of load sub / 4)
-                rs[i & 1] = *(const float*)(scales + 1024 * (sub >> 2) + 16 * (sub & 3) * scale_row);
-            };
-            rows(0);
+            const int after = buf + 1 == ST ? 0 : buf + 1;
+            f16x8 wf[BF16 ? 1 : NS][4];
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
-                const uint8_t* w = st + (T::kBM + 16 * NS * wn + 4 * T::kCols * (n / T::P) + 4 * (n % T::P)) * kFp8Block;
-                wl[n] = *(const i32x4*)(w + wpiece0);
-                wh[n] = *(const i32x4*)(w + wpiece1);
-                if (TAIL) {
-                    if (16 * fg >= p.K - b * kFp8Block) wl[n] = i32x4{};
-                    if (16 * (fg + 4) >= p.K - b * kFp8Block) wh[n] = i32x4{};
+                if (LAST) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (16 * (fg + (c & 4)) >= p.K - b * kFp8Block) wv[n][c] = 0;
+                }
+                if constexpr (!BF16) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) wf[n][q] = fp8_to_f16(wv[n][2 * q], wv[n][2 * q + 1]);
                 }
             }
-            f16x8 wf[BF16 ? 1 : NS][4];
-            if constexpr (!BF16) {
+            f16x8 af[BF16 ? 1 : kLate][4];
+            auto convert = [&](int i, int to) {
+                if constexpr (!BF16) {
 #pragma unroll
-                for (int n = 0; n < NS; ++n) {
-                    wf[n][0] = fp8_to_f16(wl[n][0], wl[n][1]);
-                    wf[n][1] = fp8_to_f16(wl[n][2], wl[n][3]);
-                    wf[n][2] = fp8_to_f16(wh[n][0], wh[n][1]);
-                    wf[n][3] = fp8_to_f16(wh[n][2], wh[n][3]);
+                    for (int q = 0; q < 4; ++q) af[to][q] = fp8_to_f16(av[slot(i)][2 * q], av[slot(i)][2 * q + 1]);
                 }
-            }
-            const bool more = !TAIL && b + ST - 1 < KB;
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                if (i + 1 < MI) rows(i + 1);
-                const float s = ws * rs[i & 1];
+            };
+            auto product = [&](int i, int n, int from) {
+                f32x4 t;
                 if constexpr (BF16) {
-                    const i32x8 af = __builtin_shufflevector(al[i & 1], ah[i & 1], 0, 1, 2, 3, 4, 5, 6, 7);
-                    f32x4 t[NS];
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-                        t[n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            __builtin_shufflevector(wl[n], wh[n], 0, 1, 2, 3, 4, 5, 6, 7), af, f32x4{}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(s, t[n][c], acc[i][n][c]);
+                    t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[n], av[slot(i)], f32x4{}, 0, 0, 0, 0, 0, 0);
                 } else {
-                    const f16x8 a0 = fp8_to_f16(al[i & 1][0], al[i & 1][1]), a1 = fp8_to_f16(al[i & 1][2], al[i & 1][3]);
-                    const f16x8 a2 = fp8_to_f16(ah[i & 1][0], ah[i & 1][1]), a3 = fp8_to_f16(ah[i & 1][2], ah[i & 1][3]);
-#pragma unroll
-                    for (int n = 0; n < NS; ++n) {
-                        f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][0], a0, f32x4{}, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][1], a1, t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][2], a2, t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][3], a3, t, 0, 0, 0);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(s, t[c], acc[i][n][c]);
-                    }
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][0], af[from][0], f32x4{}, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][1], af[from][1], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][2], af[from][2], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][3], af[from][3], t, 0, 0, 0);
                 }
-                // a later step's loads: with two buffers at once, so that they have this step to
-                // land; with more, a few after each subtile
-                if (!TAIL && more) {
-                    if (i == 0 && (b + ST - 1) % 4 == 0) load_scales(b + ST - 1);
+                return t;
+            };
+            auto add = [&](int i, int n, float s, f32x4 t) {
 #pragma unroll
-                    for (int l = 0; l < T::kLoads; ++l)
-                        if (ST == 2 ? i == 0 : l >= i * T::kLoads / MI && l < (i + 1) * T::kLoads / MI) load(l, b + ST - 1, next);
-                }
+                for (int c = 0; c < 4; ++c) acc[i][n][c] = fmaf(s, t[c], acc[i][n][c]);
+            };
+#pragma unroll
+            for (int i = 0; i < MI - kLate; ++i) {
+                rows(i + 1, b, buf);
+                if (i == 0 && !LAST && kFirst < T::kLoads && b > 0 && b - 1 + ST < KB)
+                    load(b - 1 + ST, buf ? buf - 1 : ST - 1, kFirst, T::kLoads);
+                const float s = ws * rs[slot(i)];
+                convert(i, 0);
+                f32x4 t[NS];
+#pragma unroll
+                for (int n = 0; n < NS; ++n) t[n] = product(i, n, 0);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) add(i, n, s, t[n]);
                 if (!BF16) __builtin_amdgcn_sched_barrier(0);  // (loads moved up from the next subtile would spill)
             }
-            buf = buf + 1 == ST ? 0 : buf + 1;
-            next = next + 1 == ST ? 0 : next + 1;
+            if (kLate == 2) rows(MI - 1, b, buf);
+            if (!LAST) {
+                // step b + 1 has landed (at most the ST - 2 after it are in flight; a wave's scale loads come before its
+                // stage's) ...
+#pragma unroll
+                for (int i = 0; i < MI - kLate; ++i)
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) asm volatile("" : "+v"(acc[i][n]));  // (sums sunk past the barrier would spill)
+                __builtin_amdgcn_sched_barrier(0);
+                if (b + ST - 1 < KB) __builtin_amdgcn_s_waitcnt(vm_wait((ST - 2) * T::kLoads));
+                else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+                lds_barrier();  // ... for every wave, and step b's buffer is no longer read
+                __builtin_amdgcn_sched_barrier(0);
+                if (b + ST < KB) load(b + ST, buf, 0, kFirst);
+                if (MI > 1) rows(0, b + 1, after);
+            }
+            float s[kLate];
+#pragma unroll
+            for (int j = 0; j < kLate; ++j) {
+                s[j] = ws * rs[slot(MI - kLate + j)];
+                convert(MI - kLate + j, j);
+            }
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                f32x4 t[kLate];
+#pragma unroll
+                for (int j = 0; j < kLate; ++j) t[j] = product(MI - kLate + j, n, j);
+                if (!LAST) weights(n, after);
+#pragma unroll
+                for (int j = 0; j < kLate; ++j) add(MI - kLate + j, n, s[j], t[j]);
+            }
+            if (!LAST && MI == 1) rows(0, b + 1, after);
+            buf = after;
         };
-        const int whole = p.K / kFp8Block;
-        for (int b = 0; b < whole; ++b) step(b, std::false_type{});
-        if (whole < KB) step(whole, std::true_type{});
+        // step 0
+        if (ST < KB) __builtin_amdgcn_s_waitcnt(vm_wait((ST - 1) * T::kLoads));
+        else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+        lds_barrier();
+        rows(0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) weights(n, 0);
+        for (int b = 0; b + 1 < KB; ++b) step(b, std::false_type{});
+        step(KB - 1, std::true_type{});
     };
-    load_scales(0);
 #pragma unroll
-    for (int b = 0; b < ST - 1; ++b)
-        if (b < KB)
-#pragma unroll
-            for (int l = 0; l < T::kLoads; ++l) load(l, b, b);
+    for (int b = 0; b < ST; ++b)
+        if (b < KB) load(b, b, 0, T::kLoads);
     const int subs = (nrows + 15) >> 4;                     // subtiles with rows
     const int mine = subs > wm ? (subs - wm + WM - 1) / WM : 0;  // ... of this wave
     constexpr int kHalf = MS / 2 > 1 ? MS / 2 : 1, kQuarter = MS / 4 > 1 ? MS / 4 : 1;
