@@ -648,39 +648,44 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         return p.offsets || p.R <= 16 ? launch_stream<1, 4>(p, bf16, stream) : launch_stream<2, 2>(p, bf16, stream);
     if (!p.offsets) {
         // The largest tile that gives every CU a workgroup.  Rows x 4096 x 4096, bf16, us with tiles of
-        // 256x256 / 128x256 / 64x128 / 64x64: 4096 rows 68 / 79 / 99 / 125, 2048 59 / 40 / 51 / 65,
-        // 1024 58 / 35 / 27 / 37, 256 56 / 34 / 19 / 17.
+        // 256x256 / 128x256 / 64x128 / 32x128: 4096 rows 63 / 76 / 97, 2048 52 / 38 / 50 / 65, 1024 51 / 34 / 26 / 40,
+        // 256 51 / 33 / 18 / 15.
         if (wgs(256, 256) >= kFp8Cus) return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
         if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
-        return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
+        return launch_tile<1, 4, 2, 2, 3>(p, bf16, stream);
     }
-    // By the rows an expert has on average: the tile that holds most experts' rows with few rows to
-    // spare.  256 experts of 1024 x 2048, us with 256x256 / 160x128 / 128x256 / 64x128, bf16: 32 rows
-    // 123 / 107 / 104 / 99 and 64 rows 133 / 121 / 114 / 125 (all through the caches), 93 rows
-    // 130 / 122 / 111, 128 rows 150 / 138 / 151, 156 rows 162 / 166 / 185, 187 rows 177 / 209 / 202; f32:
-    // 93 rows 165 / 180 / 166, 128 rows 219 / 196 / 218, 156 rows 261 / 235 / 261, 187 rows 266 / 300 /
-    // 306; 64 experts of 1536 x 1536: 281 rows 87 / 79 / 90, f32 147 / 116 / 134.
     const int64_t mean = p.R / p.E;
     // bf16 results larger than an L2 past the caches where the weights go past them: 32768 rows 150 / 142 us,
     // 4096 rows (8 MB) 89 / 85, the quantization after them no slower; 512 rows (1 MB) 69 / 72; f32 197 / 201.
     p.stream_out = bf16 && mean <= 256 && (int64_t)p.R * p.N * 2 > (4 << 20);
+    // By the rows an expert has on average: the tile that holds most experts' rows with few rows to spare.  Four
+    // layers' weights in turn, us with 256x256 / 160x128 / 128x256 / 128x128 / 64x128; 256 experts of 1024 x 2048, bf16:
+    // 32 rows 106 / 97 / 92 / 94 / 88, 64 rows 112 / 109 / 100 / 106 / 122, 93 rows 125 / 125 / 112 / 119, 128 rows 138 /
+    // 137 / 150 / 160, 156 rows 159 / 168 / 186 / 193, 187 rows 167 / 212 / 199 / 205; 128 of 1408 x 2816, 125 rows 138 /
+    // 130 / 145 / 149; f32: 64 rows 150 / 144 / 139 / 135 / 145, 128 rows 220 / 195 / 216 / 208; 128 of 2816 x 704, 62
+    // rows 99 / 89 / 96 / 87 / 90; through the caches 256 experts, 156 rows 261 / 235, 187 rows 266 / 300; 64 of
+    // 1536 x 1536, 281 rows, bf16 87 / 79 / 90, f32 147 / 116 / 134.
     if (mean >= 110) {
-        if (((mean > 160 && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
+        if (((mean > (bf16 ? 140 : 160) && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
             return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
-    } else if (mean >= 56 && wgs(128, 256) >= kFp8Cus) {
-        return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
+    } else if (mean >= 56) {
+        if (bf16 && wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
+        if (!bf16 && wgs(128, 128) >= kFp8Cus) return launch_tile<2, 2, 4, 4, 2>(p, bf16, stream);
     }
-    // Weights streamed for few rows: small tiles, many loads in flight, unless K is soon over.  Four layers'
-    // weights in turn, us with 32x64 in four buffers / 64x128 in three / in two: 256 experts of 1024 x 2048, 2
-    // tokens 8.4 / 11.2 / 17.1, 10 tokens 25 / 28 / 25, 64 69 / 71 / 76, 512 89 / 90 / 93; 32 of 2048 x 4096,
-    // 100 tokens 51 / 59 / 61; 128 of 2816 x 704, 64 tokens 54 / 54 / 53; 256 of 2048 x 512, 64 tokens 45 / 43 /
-    // 40, 211 tokens 52 / 51 / 49.
-    if (mean < 20 && p.KB >= 8) return launch_tile<1, 4, 2, 1, 4>(p, bf16, stream);
+    // Weights streamed for few rows: small tiles, many loads in flight, unless K is soon over; up to 20 rows also where
+    // there would be few large tiles.  Us with 32x64 in four buffers / in three / 64x128 in three / in two: 256 experts
+    // of 1024 x 2048, 2 tokens 8.4 / 9.6 / 10.8 / 15.9, 10 tokens 24.7 / 26.1 / 27.5 / 25.6, 256 82 / 82 / 84 / 88, 512
+    // 88 / 89 / 86 / 88; 32 of 2048 x 4096, 100 tokens 48 / 53 / 57 / 61; 128 of 2816 x 704 f32, 64 tokens 52 / 50 / 52 /
+    // 52, 211 57 / 55 / 56 / 58, 500 76 / 74 / 65 / 66; 256 of 2048 x 512, 64 tokens 42 / 40 / 43 / 39, 211 53 / 48 /
+    // 50 / 47.
+    if ((mean < 12 || (mean < 20 && wgs(64, 128) < 4 * kFp8Cus)) && p.KB >= 8)
+        return launch_tile<1, 4, 2, 1, 4>(p, bf16, stream);
+    if (mean < 16 && p.KB > 4 && p.KB < 8) return launch_tile<1, 4, 2, 1, 3>(p, bf16, stream);
     if (wgs(64, 128) >= kFp8Cus)
         return p.KB <= 4 ? launch_tile<1, 4, 4, 2, 2>(p, bf16, stream) : launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
-    return launch_tile<1, 4, 4, 1, 3>(p, bf16, stream);
+    return launch_tile<1, 4, 2, 2, 3>(p, bf16, stream);
 }
 
 }  // namespace qmoe

@@ -444,7 +444,7 @@ def test_matmul_nan_stays_in_its_row(gpu, M, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("E,R,N,K", [(0, 4100, 4104, 144), (0, 2050, 4100, 272), (0, 600, 2100, 528), (0, 300, 520, 144),
                                      (8, 1500, 5128, 144), (8, 2000, 1704, 272), (16, 1280, 2696, 144), (24, 700, 2000, 656),
-                                     (8, 900, 1000, 1040), (40, 600, 1000, 1040), (40, 700, 900, 400), (2, 4500, 3000, 128), (300, 2400, 260, 256), (70, 20000, 256, 528)])
+                                     (8, 900, 1000, 1040), (40, 600, 1000, 1040), (40, 700, 900, 400), (60, 700, 900, 656), (2, 4500, 3000, 128), (300, 2400, 260, 256), (70, 20000, 256, 528)])
 def test_matmul_tile_sizes(gpu, E, R, N, K, dtype):
     """Every tile, at its edges: sizes that fill the device, odd rows, columns and blocks; against 64 bits on
     the device, the whole result."""
