@@ -22,20 +22,23 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // 16 lanes take a block, 8 columns each (one or two 16-byte loads), so a wave
 // covers 512 columns; no LDS, no barrier.  Bound by memory: 4096 x 2048 f32 (42 MB) 8.2
 // us, 5.1 TB/s (0.5 of it for the exact quotients); 32768 x 512 SwiGLU of bf16 (84 MB)
-// 19.9 us, 4.2 TB/s, level with its arithmetic (21.0 with a division per value).
+// 19.0 us, 4.4 TB/s, level with its arithmetic (21.0 with expf, 22 with a division a value).
 // ---------------------------------------------------------------------------
 // g sigmoid(z) u.  Every rounding takes some values that lie next to an e4m3 border to its
-// other side: 1 / (1 + e) is an approximate reciprocal, whose remainder (with what 1 + e
-// dropped) corrects the quotient within the product with u.
+// other side: exp(-z) is the hardware's 2^t times what t = -z / ln 2 lost in rounding, and
+// 1 / (1 + e) an approximate reciprocal, whose remainder corrects the quotient within the
+// product with u (taken in the order in which its large terms cancel exactly).
 __device__ __forceinline__ float fp8_act(int act, float g, float u) {
     if (act == kFp8ActNone) return g;
     // gelu's tanh form is g sigmoid(2 z) with z = sqrt(2/pi) (g + 0.044715 g^3)
     const float z = act == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
-    const float e = expf(-z), d = 1.0f + e;
-    if (!(d < 1e30f)) return g / d * u;  // (and NaN)
-    const float low = e > 1.0f ? 1.0f - (d - e) : e - (d - 1.0f);
-    const float r = __builtin_amdgcn_rcpf(d), q = g * r;
-    return fmaf(q, u, fmaf(-q, low, fmaf(-q, d, g)) * r * u);
+    const float t = z * -1.44269504f;
+    const float e0 = __builtin_amdgcn_exp2f(t);
+    if (!(e0 < 1e30f)) return g / (1.0f + expf(-z)) * u;  // (and NaN)
+    const float e = fmaf(e0, fmaf(-t, -1.90465421e-9f, fmaf(-t, 0.693147182f, -z)), e0);  // ln 2 = 0.693147182 - 1.9e-9
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), q = g * r;
+    const float rest = e < 1.0f ? fmaf(-q, e, g - q) : fmaf(-q, e, g) - q;
+    return fmaf(q, u, rest * r * u);
 }
 
 template <bool BF16, bool WHOLE>
