@@ -24,21 +24,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // us, 5.1 TB/s (0.5 of it for the exact quotients); 32768 x 512 SwiGLU of bf16 (84 MB)
 // 19.0 us, 4.4 TB/s, level with its arithmetic (21.0 with expf, 22 with a division a value).
 // ---------------------------------------------------------------------------
-// g sigmoid(z) u.  Every rounding takes some values that lie next to an e4m3 border to its
-// other side: exp(-z) is the hardware's 2^t times what t = -z / ln 2 lost in rounding, and
-// 1 / (1 + e) an approximate reciprocal, whose remainder corrects the quotient within the
-// product with u (taken in the order in which its large terms cancel exactly).
 __device__ __forceinline__ float fp8_act(int act, float g, float u) {
-    if (act == kFp8ActNone) return g;
     // gelu's tanh form is g sigmoid(2 z) with z = sqrt(2/pi) (g + 0.044715 g^3)
-    const float z = act == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
-    const float t = z * -1.44269504f;
-    const float e0 = __builtin_amdgcn_exp2f(t);
-    if (!(e0 < 1e30f)) return g / (1.0f + expf(-z)) * u;  // (and NaN)
-    const float e = fmaf(e0, fmaf(-t, -1.90465421e-9f, fmaf(-t, 0.693147182f, -z)), e0);  // ln 2 = 0.693147182 - 1.9e-9
-    const float r = __builtin_amdgcn_rcpf(1.0f + e), q = g * r;
-    const float rest = e < 1.0f ? fmaf(-q, e, g - q) : fmaf(-q, e, g) - q;
-    return fmaf(q, u, rest * r * u);
+    return sigmoid_product(g, act == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g), u);
 }
 
 template <bool BF16, bool WHOLE>

@@ -127,6 +127,20 @@ __device__ __forceinline__ float fp8_block_max(const float (&v)[8]) {
     }
     return __builtin_bit_cast(float, m);
 }
+// a sigmoid(z) u, to about one rounding (every rounding takes some values that lie next to an
+// e4m3 border to its other side): exp(-z) is the hardware's 2^t times what t = -z / ln 2 lost
+// in rounding, and 1 / (1 + e) an approximate reciprocal, whose remainder corrects the quotient
+// within the product with u (taken in the order in which its large terms cancel exactly).
+__device__ __forceinline__ float sigmoid_product(float a, float z, float u) {
+    const float t = z * -1.44269504f;
+    const float e0 = __builtin_amdgcn_exp2f(t);
+    const float e = fmaf(e0, fmaf(-t, -1.90465421e-9f, fmaf(-t, 0.693147182f, -z)), e0);  // ln 2 = 0.693147182 - 1.9e-9
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), q = a * r;
+    const float rest = e < 1.0f ? fmaf(-q, e, a - q) : fmaf(-q, e, a) - q;
+    const float v = fmaf(q, u, rest * r * u);
+    // (the ends of the exponential, infinite operands, NaN)
+    return e0 < 1e30f && __builtin_fabsf(v) < __builtin_huge_valf() ? v : a / (1.0f + expf(-z)) * u;
+}
 // A value that rounds to e4m3 as the exact v * 448 / m does (ties to even): p = v * f32(448 /
 // m) is within two of its last places of that, and next to e4m3's border t (the middle of
 // two neighbours) the side is decided by |v| 448 against t m, both exact in f64.

@@ -339,6 +339,23 @@ def test_quantize_activation(gpu, R, C, act, dtype):
     check_fp8(q, s, v, 460 * U32, act)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+def test_quantize_activation_non_finite(gpu, act):
+    """An infinite product gives its block an infinite scale, NaN a NaN one; a far negative gate gives zeros."""
+    x = torch.ones(6, 2, 256)
+    x[0, 0, 3], x[1, 1, 130], x[2, 0, 200], x[3, 1, 7] = math.inf, -math.inf, -1000.0, math.nan
+    x[4, 0, :128] = -1000.0
+    x[5, 0, 1], x[5, 1, 1] = 3e38, 3e38
+    _, s = (t.cpu() for t in qa.fp8_quantize(x.view(6, 512).to(gpu), act=act))
+    one = s[2, 0]
+    assert torch.isfinite(one) and one > 0
+    assert math.isinf(s[0, 0]) and math.isinf(s[1, 1]) and math.isnan(s[3, 0]) and math.isinf(s[5, 0])
+    assert s[4, 0] == torch.tensor(1e-30) / 448
+    for r, b in ((0, 1), (1, 0), (2, 1), (3, 1), (4, 1), (5, 1)):
+        assert s[r, b] == one
+
+
 # ---- products --------------------------------------------------------------------------------------
 
 def check_product(y, a, s, w, sw, dtype, what=""):
