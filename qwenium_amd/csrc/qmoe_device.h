@@ -64,21 +64,26 @@ __device__ __forceinline__ void store1(void* y, uint64_t at, float v) {
     if (BF16) ((uint16_t*)y)[at] = (uint16_t)f32_pack_bf16(v, 0.0f);
     else ((float*)y)[at] = v;
 }
+// (bf16 becomes f32 behind the branch: inside, each load would be waited for there)
 template <bool BF16, bool WHOLE>
 __device__ __forceinline__ void load8(const void* x, uint64_t at, int n, float (&v)[8]) {
-    if (WHOLE || n >= 8) {
-        if constexpr (BF16) {
-            const u16x8a2 r = *(const u16x8a2*)((const uint16_t*)x + at);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(r[i]);
+    if constexpr (BF16) {
+        u16x8a2 r;
+        if (WHOLE || n >= 8) {
+            r = *(const u16x8a2*)((const uint16_t*)x + at);
         } else {
-            const f32x4a4 r = *(const f32x4a4*)((const float*)x + at), s = *(const f32x4a4*)((const float*)x + at + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = r[i], v[4 + i] = s[i];
+            for (int i = 0; i < 8; ++i) r[i] = i < n ? ((const uint16_t*)x)[at + i] : (uint16_t)0;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = bf16_to_f32(r[i]);
+    } else if (WHOLE || n >= 8) {
+        const f32x4a4 r = *(const f32x4a4*)((const float*)x + at), s = *(const f32x4a4*)((const float*)x + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = r[i], v[4 + i] = s[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? load1<BF16>(x, at + i) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? load1<false>(x, at + i) : 0.0f;
     }
 }
 template <bool BF16, bool WHOLE>

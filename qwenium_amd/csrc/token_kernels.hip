@@ -236,7 +236,7 @@ hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_col
 // y[t] = residual[t] + sum_j w[t][j] ys[place[t][j]], j in order in f32, rounded
 // once (w null: ones, the gather's gradient).  Assignments without a place add
 // nothing.  8 columns a thread, the rows of 8 assignments in flight: 4096 x 8 rows of
-// 4 KB and a residual (168 MB) 42 us, 4.0 TB/s.
+// 4 KB and a residual (168 MB) 38 us, 4.4 TB/s (with a branch around each load 42).
 // ---------------------------------------------------------------------------
 template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, int top_k, int R, const int32_t* place,
@@ -254,7 +254,8 @@ __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, i
             const int p = place[a];
             has[j] = j0 + j < top_k && p >= 0 && p < R;
             wj[j] = w ? w[a] : 1.0f;
-            if (has[j]) load8<BF16, WHOLE>(ys, (uint64_t)p * H + c0, n, v[j]);
+            // (without a branch around it: the loads go out together)
+            load8<BF16, WHOLE>(ys, (uint64_t)(has[j] ? p : 0) * H + c0, n, v[j]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -288,7 +289,7 @@ hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H,
 // shared between workgroups: a thread adds its columns' products in turn (8
 // columns and 8 assignments in flight), then the tree over its wave's lanes and
 // the waves in turn.  Rows behind the last expert's get zeros.  2000 x 6 rows of 6 KB
-// (160 MB): 34 us, 4.7 TB/s.
+// (160 MB): 34 us, 4.7 TB/s; 4096 x 8 of 4 KB 56 us (with a branch around each load 78).
 // ---------------------------------------------------------------------------
 template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, con
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int p = j0 + j < top_k ? place[t * top_k + j0 + j] : -1;
-                if (p >= 0 && p < R) load8<BF16, WHOLE>(ys, (uint64_t)p * H + c0, n, v[j]);
+                load8<BF16, WHOLE>(ys, (uint64_t)(p >= 0 && p < R ? p : 0) * H + c0, n, v[j]);  // (no branch, as above)
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
