@@ -357,7 +357,8 @@ enum qmoe_fp8_act {
  * or the activation of x's two halves (x is then [n_rows][2 n_cols], gate columns
  * first).  Per block of 128 columns (the last may be shorter) m = the largest |v|,
  * at least 1e-30: scale = m / 448, q = e4m3(v * 448 / m) rounded once, ties to even.  A
- * block with a NaN has a NaN scale; one with an infinity an infinite scale. */
+ * block with a NaN has a NaN scale; one with an infinity an infinite scale.  Fewer than
+ * 2^28 blocks. */
 int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_cols, int32_t act,
                       uint8_t* q, float* scale, void* hip_stream);
 
@@ -392,7 +393,7 @@ int qmoe_sort_tokens(const int32_t* topk_idx, int32_t n_tokens, int32_t top_k, i
                      int32_t* offsets, int32_t* rows, int32_t* tokens, int32_t* place, void* hip_stream);
 /* y[place[t][j]] = x[t], elements of elem_bytes (1, 2 or 4): the rows in the
  * experts' order; rows from offsets[n_experts] on are zeros.  Its gradient is
- * qmoe_combine_tokens with w and residual NULL. */
+ * qmoe_combine_tokens with w and residual NULL.  n_tokens < 2^22 (here and below). */
 int qmoe_gather_tokens(const void* x, int32_t elem_bytes, int32_t n_tokens, int32_t n_cols, int32_t top_k,
                        int32_t n_experts, const int32_t* offsets, const int32_t* place, void* y, void* hip_stream);
 /* y[t] = residual[t] + sum_j w[t][j] ys[place[t][j]], j in order in f32, rounded

@@ -61,7 +61,7 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
                                hipStream_t stream) {
     const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
     if (blocks <= 0) return hipSuccess;
-    if (blocks > 0xffffffffll) return hipErrorInvalidValue;
+    if (blocks >= 1ll << 28) return hipErrorInvalidValue;  // (16 threads each, below 2^32 a launch)
     const bool whole = cols % 8 == 0;
     const dim3 grid((unsigned)((blocks + 15) / 16));
 #define QMOE_Q8(B, V) hipLaunchKernelGGL((k_fp8_quantize<B, V>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale)
@@ -608,7 +608,7 @@ static int64_t fp8_max_tiles(const Fp8Product& p, int tile) {
 template <int MT, int U>
 static hipError_t launch_stream(const Fp8Product& p, bool bf16, hipStream_t stream) {
     const int64_t blocks = fp8_max_tiles(p, 16 * MT) * ((p.N + 15) / 16);
-    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    if (blocks >= 1ll << 24) return hipErrorInvalidValue;  // (below 2^32 threads)
     if (bf16) hipLaunchKernelGGL((k_fp8_stream<MT, U, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((k_fp8_stream<MT, U, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     return hipGetLastError();
@@ -619,7 +619,7 @@ static hipError_t launch_tile_as(const Fp8Product& p, hipStream_t stream) {
     using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
     const int64_t tiles = fp8_max_tiles(p, T::kBM), nt = (p.N + T::kBN - 1) / T::kBN;
     const int64_t blocks = p.offsets ? (tiles + 7) / 8 * 8 * nt : (tiles * nt + 7) / 8 * 8;
-    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    if (blocks * (64 * T::kWaves) >= 1ll << 32) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_fp8_tile<WM, WN, MS, NS, ST, BF16>), dim3((unsigned)blocks), dim3(64 * T::kWaves), T::kLds, stream, p);
     return hipGetLastError();
 }

@@ -70,6 +70,9 @@ int check_tokens(int32_t n_tokens, int32_t top_k) {
     return in_range("n_tokens * top_k", (int64_t)n_tokens * top_k, 0, 1 << 30);
 }
 
+// A launch holds below 2^32 threads; a row takes up to 1024 (16 a block of the quantization).
+constexpr int64_t kMaxRowLaunch = (1 << 22) - 1, kMaxBlocks = (1 << 28) - 1;
+
 #define QMOE_TRY(expr)                   \
     do {                                 \
         if (int rc_ = (expr)) return rc_; \
@@ -86,7 +89,7 @@ int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_c
     QMOE_TRY(in_range("n_rows", n_rows, 0, INT32_MAX));
     QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 28));
     QMOE_TRY(in_range("act", act, QMOE_FP8_ACT_NONE, QMOE_FP8_ACT_GEGLU));
-    QMOE_TRY(in_range("n_rows * ceil(n_cols/128)", (int64_t)n_rows * ((n_cols + 127) / 128), 0, 0xffffffffll));
+    QMOE_TRY(in_range("n_rows * ceil(n_cols/128)", (int64_t)n_rows * ((n_cols + 127) / 128), 0, kMaxBlocks));
     if (n_rows == 0) return QMOE_OK;
     QMOE_TRY(need("x", x));
     QMOE_TRY(need("q", q));
@@ -177,6 +180,7 @@ int qmoe_gather_tokens(const void* x, int32_t elem_bytes, int32_t n_tokens, int3
                        int32_t n_experts, const int32_t* offsets, const int32_t* place, void* y, void* hip_stream) {
     qmoe::clear_error();
     QMOE_TRY(check_tokens(n_tokens, top_k));
+    QMOE_TRY(in_range("n_tokens", n_tokens, 0, kMaxRowLaunch));
     QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     QMOE_TRY(in_range("n_experts", n_experts, 1, 1024));
     if (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4) return bad_value("elem_bytes", "1, 2 or 4", str(elem_bytes));
@@ -202,6 +206,7 @@ int qmoe_combine_tokens(const void* ys, int32_t x_type, int32_t n_tokens, int32_
     qmoe::clear_error();
     QMOE_TRY(row_type("x_type", x_type));
     QMOE_TRY(check_tokens(n_tokens, top_k));
+    QMOE_TRY(in_range("n_tokens", n_tokens, 0, kMaxRowLaunch));
     QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     if (n_tokens == 0) return QMOE_OK;
     QMOE_TRY(need("ys", ys));
@@ -226,6 +231,7 @@ int qmoe_combine_tokens_backward(const void* dy, const void* ys, int32_t x_type,
     qmoe::clear_error();
     QMOE_TRY(row_type("x_type", x_type));
     QMOE_TRY(check_tokens(n_tokens, top_k));
+    QMOE_TRY(in_range("n_tokens", n_tokens, 0, kMaxRowLaunch));
     QMOE_TRY(in_range("n_cols", n_cols, 1, 1 << 20));
     QMOE_TRY(in_range("n_experts", n_experts, 1, 1024));
     if (n_tokens == 0) return QMOE_OK;
@@ -256,7 +262,7 @@ int qmoe_residual_norm(const qmoe_norm_args* a, int32_t n_tokens, int32_t n_embd
     qmoe::clear_error();
     if (!a) return set_error(QMOE_ERR_NULL, "qmoe: args expected non-null, got null");
     QMOE_TRY(row_type("x_type", a->x_type));
-    QMOE_TRY(in_range("n_tokens", n_tokens, 0, INT32_MAX));
+    QMOE_TRY(in_range("n_tokens", n_tokens, 0, kMaxRowLaunch));
     QMOE_TRY(in_range("n_embd", n_embd, 1, 16384));
     QMOE_TRY(in_range("gate_act", a->gate_act, QMOE_GATE_NONE, QMOE_GATE_SILU));
     if (!(a->eps >= 0.0f) || std::isinf(a->eps)) return bad_value("eps", "a number >= 0", std::to_string(a->eps));

@@ -123,7 +123,7 @@ def rc_quantize(x=FAKE, t=TYPE_F32, R=4, C=256, act=0, q=FAKE + MIB, s=FAKE + 2 
     (dict(x=FAKE + 2), QMOE_ERR_VALUE, "aligned"), (dict(q=FAKE), QMOE_ERR_VALUE, "distinct"),
     (dict(q=FAKE + 4095), QMOE_ERR_VALUE, "q expected a buffer distinct from x"), (dict(s=FAKE - 28), QMOE_ERR_VALUE, "distinct"),
     (dict(s=FAKE + MIB + 1020), QMOE_ERR_VALUE, "scale expected a buffer distinct from q"),
-    (dict(R=2 ** 31 - 1, C=2 ** 28), QMOE_ERR_VALUE, "ceil(n_cols/128)"),
+    (dict(R=2 ** 31 - 1, C=2 ** 28), QMOE_ERR_VALUE, "ceil(n_cols/128)"), (dict(R=2 ** 28, C=1), QMOE_ERR_VALUE, "ceil(n_cols/128)"),
 ])
 def test_quantize_refusals(kw, code, needle):
     assert rc_quantize(**kw) == code
@@ -184,6 +184,18 @@ def test_token_refusals():
     assert L.qmoe_combine_tokens(None, TYPE_F32, 4, 8, 2, b, c, d, e, None) == QMOE_ERR_NULL
     assert L.qmoe_combine_tokens_backward(a, b, TYPE_F32, 4, 8, 2, 4, c, d, e, a, a + 64, None) == QMOE_ERR_VALUE
     assert L.qmoe_combine_tokens_backward(a, b, TYPE_F32, 4, 8, 2, 4, c, d, None, e, a + 64, None) == QMOE_ERR_NULL
+
+
+def test_rows_of_one_launch():
+    """A launch holds below 2^32 threads: more rows are refused."""
+    L, T = _lib.lib(), 1 << 22
+    a, b, c, d, e, f, g = (FAKE + (i << 40) for i in range(7))
+    assert L.qmoe_gather_tokens(a, 4, T, 8, 1, 4, b, c, d, None) == QMOE_ERR_VALUE and "n_tokens" in _lib.last_error()
+    assert L.qmoe_combine_tokens(a, TYPE_F32, T, 8, 1, b, c, d, e, None) == QMOE_ERR_VALUE and "n_tokens" in _lib.last_error()
+    assert L.qmoe_combine_tokens_backward(a, b, TYPE_F32, T, 8, 1, 4, c, d, e, f, g, None) == QMOE_ERR_VALUE
+    assert "n_tokens" in _lib.last_error()
+    norm = norm_args(x=a, y=b, x_out=c, h=d)
+    assert L.qmoe_residual_norm(ctypes.byref(norm), T, 8, None) == QMOE_ERR_VALUE and "n_tokens" in _lib.last_error()
 
 
 def norm_args(**kw):
