@@ -4,6 +4,8 @@
 #include "qmoe_device.h"
 #include "qmoe_internal.h"
 
+#include <type_traits>
+
 namespace qmoe {
 
 // ---------------------------------------------------------------------------
@@ -193,10 +195,13 @@ static void row_grid(int n_tokens, int64_t pieces, dim3& grid, dim3& block) {
 // top_k times (reading by sorted row would read it top_k times).  Rows behind the
 // last expert's belong to no token: zeros, by the token with those list indices.
 // 4096 rows of 4 KB, 8 times (151 MB): 27 us, 5.6 TB/s.  A thread takes 16 bytes; a
-// row's last 16 may overlap the ones before (the same bytes written twice).  V: 16 bytes, or single bytes for rows shorter than that.
+// row's last 16 may overlap the ones before (the same bytes written twice).  V: 16 bytes, or
+// single bytes for rows shorter than that.  NT: past the caches, where the rows are more
+// than these hold (8192 x 2 rows of 8 KB 40 -> 31 us).
 // ---------------------------------------------------------------------------
 typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));
-template <typename V>
+constexpr int64_t kStreamBytes = 32 << 20;  // the L2s of 8 XCDs
+template <typename V, bool NT>
 __global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int bytes, int top_k, int R, const int32_t* total,
                                                        const int32_t* place, uint8_t* y) {
     constexpr int kSize = sizeof(V);
@@ -210,7 +215,10 @@ __global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int byt
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
         const int p = pl[j];
-        if (p >= 0 && p < R) *(V*)(y + (uint64_t)p * bytes + i) = v;
+        if (p >= 0 && p < R) {
+            if constexpr (NT) __builtin_nontemporal_store(v, (V*)(y + (uint64_t)p * bytes + i));
+            else *(V*)(y + (uint64_t)p * bytes + i) = v;
+        }
         const int r = t * top_k + j;
         if (r >= last) *(V*)(y + (uint64_t)r * bytes + i) = V{};
     }
@@ -223,57 +231,131 @@ hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_col
     dim3 grid, block;
     row_grid(n_tokens, bytes >= 16 ? (bytes + 15) / 16 : bytes, grid, block);
     if (grid.y > 65535) return hipErrorInvalidValue;
-    if (bytes >= 16)
-        hipLaunchKernelGGL(k_gather_tokens<u32x4a1>, grid, block, 0, stream, (const uint8_t*)x, bytes, top_k, n_tokens * top_k,
-                           total, place, (uint8_t*)y);
-    else
-        hipLaunchKernelGGL(k_gather_tokens<uint8_t>, grid, block, 0, stream, (const uint8_t*)x, bytes, top_k, n_tokens * top_k,
-                           total, place, (uint8_t*)y);
+    const bool stream_out = (int64_t)n_tokens * top_k * bytes > kStreamBytes;
+#define QMOE_GATHER(...)                                                                                               \
+    hipLaunchKernelGGL((k_gather_tokens<__VA_ARGS__>), grid, block, 0, stream, (const uint8_t*)x, bytes, top_k,        \
+                       n_tokens * top_k, total, place, (uint8_t*)y)
+    if (bytes < 16) QMOE_GATHER(uint8_t, false);
+    else if (stream_out) QMOE_GATHER(u32x4a1, true);
+    else QMOE_GATHER(u32x4a1, false);
+#undef QMOE_GATHER
     return hipGetLastError();
+}
+
+// 16 bytes of a row, C elements, at the elements' alignment.  A row's last piece starts at
+// H - C: the first of its columns are its neighbour's, which alone stores them.
+template <bool BF16>
+struct Piece {
+    static constexpr int C = BF16 ? 8 : 4;
+    u32x4a2 r;
+    // of H columns from c on; NT: read once (unaligned pieces share lines)
+    template <bool WHOLE, bool NT = false>
+    __device__ __forceinline__ void load(const void* row, int c, int H) {
+        if (WHOLE || H >= C) {
+            const u32x4a2* p = (const u32x4a2*)((const uint8_t*)row + (int64_t)c * (16 / C));
+            if constexpr (WHOLE && NT) r = __builtin_nontemporal_load(p);
+            else r = *p;
+        } else {
+            float v[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) v[i] = i < H ? load1<BF16>(row, i) : 0.0f;
+            set(v);
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[C]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (BF16) r[i] = f32_pack_bf16(v[2 * i], v[2 * i + 1]);
+            else r[i] = __builtin_bit_cast(uint32_t, v[i]);
+        }
+    }
+    // the columns from c + skip on
+    template <bool WHOLE, bool NT = false>
+    __device__ __forceinline__ void store(void* row, int c, int H, int skip) const {
+        if (WHOLE || (H >= C && skip == 0)) {
+            u32x4a2* p = (u32x4a2*)((uint8_t*)row + (int64_t)c * (16 / C));
+            if constexpr (NT) __builtin_nontemporal_store(r, p);
+            else *p = r;
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (i >= skip && c + i < H) store1<BF16>(row, c + i, (*this)[i]);
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        const uint32_t v = r[BF16 ? i >> 1 : i];
+        if constexpr (BF16) return __builtin_bit_cast(float, i & 1 ? v & 0xffff0000u : v << 16);
+        else return __builtin_bit_cast(float, v);
+    }
+};
+template <bool BF16>
+__device__ __forceinline__ const void* row_at(const void* x, int64_t row, int H) {
+    return (const uint8_t*)x + row * H * (BF16 ? 2 : 4);
+}
+template <bool BF16>
+__device__ __forceinline__ void* row_at(void* x, int64_t row, int H) {
+    return (uint8_t*)x + row * H * (BF16 ? 2 : 4);
 }
 
 // ---------------------------------------------------------------------------
 // y[t] = residual[t] + sum_j w[t][j] ys[place[t][j]], j in order in f32, rounded
 // once (w null: ones, the gather's gradient).  Assignments without a place add
-// nothing.  8 columns a thread, the rows of 8 assignments in flight: 4096 x 8 rows of
-// 4 KB and a residual (168 MB) 38 us, 4.4 TB/s (with a branch around each load 42).
+// nothing.  16 bytes a thread, the rows of 8 assignments in flight, past the caches (a row
+// is read once): 4096 x 8 rows of 4 KB and a residual (168 MB), several in turn, 28.5 us,
+// 5.9 TB/s (through the caches 33.6; with a branch around each load 38).
 // ---------------------------------------------------------------------------
 template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(256) void k_combine_tokens(const void* ys, int H, int top_k, int R, const int32_t* place,
                                                         const float* w, const void* residual, void* y) {
-    const int t = blockIdx.x, c0 = 8 * (blockIdx.y * blockDim.x + threadIdx.x), n = H - c0;
-    if (n <= 0) return;
-    float s[8] = {}, res[8] = {};
-    if (residual) load8<BF16, WHOLE>(residual, (uint64_t)t * H + c0, n, res);
-    for (int j0 = 0; j0 < top_k; j0 += 8) {
-        float v[8][8], wj[8];
+    constexpr int C = Piece<BF16>::C;
+    const int t = blockIdx.x, c0 = C * (blockIdx.y * blockDim.x + threadIdx.x);
+    if (c0 >= H) return;
+    const int c = WHOLE || c0 + C <= H || H < C ? c0 : H - C;
+    float s[C] = {};
+    Piece<BF16> res;
+    if (residual) res.template load<WHOLE>(row_at<BF16>(residual, t, H), c, H);
+    // 8 assignments' rows at once (FULL: a branch around a load would hold the next one up)
+    auto add8 = [&](int j0, auto full_c) {
+        constexpr bool FULL = decltype(full_c)::value;
+        Piece<BF16> v[8];
+        float wj[8];
+        int p[8];
         bool has[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int a = t * top_k + (j0 + j < top_k ? j0 + j : 0);
-            const int p = place[a];
-            has[j] = j0 + j < top_k && p >= 0 && p < R;
+            const int a = t * top_k + (FULL || j0 + j < top_k ? j0 + j : 0);
+            p[j] = place[a];
             wj[j] = w ? w[a] : 1.0f;
-            // (without a branch around it: the loads go out together)
-            load8<BF16, WHOLE>(ys, (uint64_t)(has[j] ? p : 0) * H + c0, n, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            has[j] = (FULL || j0 + j < top_k) && p[j] >= 0 && p[j] < R;
+            if (FULL || j0 + j < top_k) v[j].template load<WHOLE, true>(row_at<BF16>(ys, has[j] ? p[j] : 0, H), c, H);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (has[j])
 #pragma unroll
-                for (int c = 0; c < 8; ++c) s[c] = fmaf(wj[j], v[j][c], s[c]);
-    }
+                for (int i = 0; i < C; ++i) s[i] = fmaf(wj[j], v[j][i], s[i]);
+    };
+    int j0 = 0;
+    for (; j0 + 8 <= top_k; j0 += 8) add8(j0, std::true_type{});
+    if (j0 < top_k) add8(j0, std::false_type{});
+    if (residual)
 #pragma unroll
-    for (int c = 0; c < 8; ++c) s[c] += res[c];
-    store8<BF16, WHOLE>(y, (uint64_t)t * H + c0, n, s);
+        for (int i = 0; i < C; ++i) s[i] += res[i];
+    Piece<BF16> out;
+    out.set(s);
+    out.template store<WHOLE>(row_at<BF16>(y, t, H), c, H, c0 - c);
 }
 
 hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H, int top_k, const int32_t* place,
                                  const float* w, const void* residual, void* y, hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const bool whole = H % 8 == 0;
+    const int C = bf16 ? 8 : 4;
+    const bool whole = H % C == 0;
     dim3 grid, block;
-    row_grid(n_tokens, ((int64_t)H + 7) / 8, grid, block);
+    row_grid(n_tokens, ((int64_t)H + C - 1) / C, grid, block);
     if (grid.y > 65535) return hipErrorInvalidValue;
 #define QMOE_COMBINE(B, V) \
     hipLaunchKernelGGL((k_combine_tokens<B, V>), grid, block, 0, stream, ys, H, top_k, n_tokens * top_k, place, w, residual, y)
@@ -286,47 +368,59 @@ hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H,
 // ---------------------------------------------------------------------------
 // The weighted sum's gradients: dys[place[t][j]] = w[t][j] dy[t] and
 // dw[t][j] = <dy[t], ys[place[t][j]]>.  One workgroup per token, so no sum is
-// shared between workgroups: a thread adds its columns' products in turn (8
-// columns and 8 assignments in flight), then the tree over its wave's lanes and
-// the waves in turn.  Rows behind the last expert's get zeros.  2000 x 6 rows of 6 KB
-// (160 MB): 34 us, 4.7 TB/s; 4096 x 8 of 4 KB 56 us (with a branch around each load 78).
+// shared between workgroups: a thread adds its columns' products in turn (16 bytes of 8
+// assignments in flight), then the tree over its wave's lanes and the waves in turn.
+// Rows behind the last expert's get zeros.  4096 x 8 rows of 4 KB (285 MB) 61.5 us, 4.6
+// TB/s; 8192 x 2 of 8 KB 85 (96 through the caches).
 // ---------------------------------------------------------------------------
-template <bool BF16, bool WHOLE>
+template <bool BF16, bool WHOLE, bool NT>
 __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
                                                              const int32_t* total, const int32_t* place, const float* w,
                                                              void* dys, float* dw) {
+    constexpr int C = Piece<BF16>::C;
     __shared__ float s_sum[8][16];
     const int t = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, nw = blockDim.x >> 6;
     const int last = *total;
     for (int j0 = 0; j0 < top_k; j0 += 8) {
-        float dot[8] = {};
-        for (int c0 = 8 * threadIdx.x; c0 < H; c0 += 8 * blockDim.x) {
-            const int n = H - c0;
-            float g[8], v[8][8];
-            load8<BF16, WHOLE>(dy, (uint64_t)t * H + c0, n, g);
+        float dot[8] = {}, wj[8];
+        int p[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int p = j0 + j < top_k ? place[t * top_k + j0 + j] : -1;
-                load8<BF16, WHOLE>(ys, (uint64_t)(p >= 0 && p < R ? p : 0) * H + c0, n, v[j]);  // (no branch, as above)
-            }
+        for (int j = 0; j < 8; ++j) {
+            const int a = t * top_k + (j0 + j < top_k ? j0 + j : 0);
+            const int at = place[a];
+            p[j] = j0 + j < top_k && at >= 0 && at < R ? at : -1;
+            wj[j] = w[a];
+        }
+        for (int c0 = C * threadIdx.x; c0 < H; c0 += C * blockDim.x) {
+            const int c = WHOLE || c0 + C <= H || H < C ? c0 : H - C;
+            Piece<BF16> dp, v[8];
+            dp.template load<WHOLE>(row_at<BF16>(dy, t, H), c, H);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < top_k) v[j].template load<WHOLE, true>(row_at<BF16>(ys, p[j] < 0 ? 0 : p[j], H), c, H);
+            float g[C];
+#pragma unroll
+            for (int i = 0; i < C; ++i) g[i] = WHOLE || i >= c0 - c ? dp[i] : 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if (j0 + j >= top_k) continue;
-                const int a = t * top_k + j0 + j, p = place[a];
-                float o[8];
-                if (p >= 0 && p < R) {
-                    const float wj = w[a];
+                Piece<BF16> out;
+                float o[C];
+                if (p[j] >= 0) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        dot[j] = fmaf(g[c], v[j][c], dot[j]);
-                        o[c] = wj * g[c];
+                    for (int i = 0; i < C; ++i) {
+                        dot[j] = fmaf(g[i], WHOLE || i >= c0 - c ? v[j][i] : 0.0f, dot[j]);
+                        o[i] = wj[j] * g[i];
                     }
-                    store8<BF16, WHOLE>(dys, (uint64_t)p * H + c0, n, o);
+                    out.set(o);
+                    out.template store<WHOLE, NT>(row_at<BF16>(dys, p[j], H), c, H, c0 - c);
                 }
+                const int a = t * top_k + j0 + j;
                 if (a >= last) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) o[c] = 0.0f;
-                    store8<BF16, WHOLE>(dys, (uint64_t)a * H + c0, n, o);
+                    for (int i = 0; i < C; ++i) o[i] = 0.0f;
+                    out.set(o);
+                    out.template store<WHOLE, NT>(row_at<BF16>(dys, a, H), c, H, c0 - c);
                 }
             }
         }
@@ -350,14 +444,17 @@ hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, 
                                      const int32_t* total, const int32_t* place, const float* w, void* dys, float* dw,
                                      hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
-    const bool whole = H % 8 == 0;
-    const int64_t pieces = ((int64_t)H + 7) / 8;
+    const int C = bf16 ? 8 : 4;
+    const bool whole = H % C == 0, stream_out = (int64_t)n_tokens * top_k * H * (16 / C) > kStreamBytes;
+    const int64_t pieces = ((int64_t)H + C - 1) / C;
     const dim3 grid(n_tokens), block((unsigned)(pieces < 1024 ? (pieces + 63) / 64 * 64 : 1024));
-#define QMOE_BWD(B, V)                                                                                                \
-    hipLaunchKernelGGL((k_combine_tokens_bwd<B, V>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, place, w, \
-                       dys, dw)
-    if (bf16) { if (whole) QMOE_BWD(true, true); else QMOE_BWD(true, false); }
-    else { if (whole) QMOE_BWD(false, true); else QMOE_BWD(false, false); }
+#define QMOE_BWD(...)                                                                                                  \
+    hipLaunchKernelGGL((k_combine_tokens_bwd<__VA_ARGS__>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, \
+                       place, w, dys, dw)
+#define QMOE_BWD_NT(B, V) do { if (stream_out) QMOE_BWD(B, V, true); else QMOE_BWD(B, V, false); } while (0)
+    if (bf16) { if (whole) QMOE_BWD_NT(true, true); else QMOE_BWD_NT(true, false); }
+    else { if (whole) QMOE_BWD_NT(false, true); else QMOE_BWD_NT(false, false); }
+#undef QMOE_BWD_NT
 #undef QMOE_BWD
     return hipGetLastError();
 }

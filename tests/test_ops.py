@@ -615,6 +615,23 @@ def test_tokens_there_and_back(gpu, T, E, k, kind, H, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [1, 3, 5, 9, 131, 1027, 2047])
+def test_combine_into_its_residual(gpu, H, dtype):
+    """Rows that end inside a 16-byte piece, the output in the residual's place: the same bits as apart."""
+    T, k, E = 37, 9, 7
+    g = gen(H)
+    o = qa.sort_tokens(torch.randint(0, E + 1, (T, k), generator=g, dtype=torch.int32).to(gpu), E)
+    ys, r = randn(g, T * k, H).to(dtype).to(gpu), randn(g, T, H).to(dtype).to(gpu)
+    w = torch.rand(T, k, generator=g).to(gpu)
+    want = qa.combine_tokens(ys, o, w, residual=r)
+    for _ in range(3):
+        y = r.clone()
+        assert qa.combine_tokens(ys, o, w, residual=y, out=y) is y
+        assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
 def test_token_gradients_against_differences(gpu):
     """L = <dy, combine(ys, w)> and L = <dxs, gather(x)> are linear in each operand, so a difference over
     any step is its derivative: (L(p + d) - L(p - d)) / 2 = <grad, d>, to the roundings of the two L."""
