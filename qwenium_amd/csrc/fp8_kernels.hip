@@ -90,11 +90,11 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // stores them together.  (Both operands take the same permutation of a block's
 // columns, which leaves its sum as it is: lane group g reads 16-byte pieces g and
 // g + 4.)
-//   Where the time goes (us): 8192 x 4096 x 4096 bf16 128 (2.1 PFLOP/s; 275 GFLOP take
+//   Where the time goes (us): 8192 x 4096 x 4096 bf16 121 (2.3 PFLOP/s; 275 GFLOP take
 // 93-104 in a library e4m3 product without block scales): the matrix instructions alone
 // 73, with the fmas of the scales 94, with the reads of LDS 103, the rest the loads to
-// it, 10 of that past the L2; f32 228 (1.2, as a library bf16 product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
-// (6.3 TB/s), 32768 rows 139-142 (613 MB: 4.3-4.4 TB/s).
+// it and the stores; f32 216 (1.3, as a library bf16 product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
+// (6.3 TB/s), 32768 rows 131-136 (613 MB: 4.5-4.7 TB/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -178,6 +178,10 @@ __device__ __forceinline__ void fp8_put(const Fp8Product& p, void* y, V v) {
     } else {
         *(V*)y = v;
     }
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t fp8_bits(float a, float b) {  // two bf16 or one f32
+    return BF16 ? f32_pack_bf16(a, b) : __builtin_bit_cast(uint32_t, a);
 }
 template <bool BF16, int C>
 __device__ __forceinline__ void fp8_store(const Fp8Product& p, int r, int n, const float (&v)[C]) {
@@ -448,7 +452,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
         constexpr int MI = decltype(mi_c)::value;
         constexpr int kLate = MI >= 4 ? 2 : 1;  // subtiles whose products come after the step's last row fragment is read
         // Eight waves load half of a stage after the barrier, half in the next step: all at once they hold each other up
-        // (8192 x 4096 x 4096 bf16 134 us, in halves 128; tiles of four waves lose 1-2% by it).
+        // (8192 x 4096 x 4096 bf16 134 us, in halves 128, both before the stores went out in lines; tiles of four waves lose 1-2% by it).
         constexpr int kFirst = T::kWaves == 8 && MI >= 4 ? (T::kLoads + 1) / 2 : T::kLoads;
         int buf = 0;
         float ws_next = scalar_load(sw);
@@ -580,18 +584,46 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     else if (mine > kQuarter) run(std::integral_constant<int, kHalf>{});
     else run(std::integral_constant<int, kQuarter>{});
 
+    // Two 64-byte pieces of a row's columns: lanes of rows 8 apart swap one of theirs, so that a store covers whole
+    // 128-byte lines (256 experts x 32768 rows 136 -> 133 us, with 93 MB written for 67 before).
+    constexpr bool kLines = NS / T::P % 2 == 0;
+    const bool lines = kLines && nw0 + 16 * NS <= p.N;
 #pragma unroll
     for (int i = 0; i < MS; ++i) {
-        const int m = 16 * (WM * i + wm) + fr;
-        if (m >= nrows) continue;
+        const int m0 = 16 * (WM * i + wm), m = m0 + fr;
+        if (m0 >= nrows) continue;
         const bool none = s_none[m];
+        auto value = [&](int n, int c) { return none ? 0.0f : acc[i][n + (c >> 2)][c & 3]; };
+        if (lines) {
+            if constexpr (kLines) {
+                const bool high = fr & 8;
+                const int ra = m0 + (fr & 7);
 #pragma unroll
-        for (int n = 0; n < NS; n += T::P) {
-            const int col = nw0 + 16 * n + T::kCols * fg;
-            float v[T::kCols];
+                for (int n = 0; n < NS; n += 2 * T::P) {
+                    uint32_t x[4], y[4];
 #pragma unroll
-            for (int c = 0; c < T::kCols; ++c) v[c] = none ? 0.0f : acc[i][n + (c >> 2)][c & 3];
-            if (col < p.N) fp8_store<BF16, T::kCols>(p, row0 + m, col, v);
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t v0 = fp8_bits<BF16>(value(n, BF16 ? 2 * c : c), BF16 ? value(n, 2 * c + 1) : 0.0f);
+                        const uint32_t v1 = fp8_bits<BF16>(value(n + T::P, BF16 ? 2 * c : c), BF16 ? value(n + T::P, 2 * c + 1) : 0.0f);
+                        const uint32_t got = __builtin_amdgcn_update_dpp(0, high ? v0 : v1, 0x128, 0xf, 0xf, false);
+                        x[c] = high ? got : v0;
+                        y[c] = high ? v1 : got;
+                    }
+                    const int col = nw0 + 16 * (high ? n + T::P : n) + T::kCols * fg;
+                    uint8_t* const to = (uint8_t*)p.y + ((uint64_t)(row0 + ra) * p.N + col) * (BF16 ? 2 : 4);
+                    if (ra < nrows) fp8_put(p, to, u32x4a2{x[0], x[1], x[2], x[3]});
+                    if (ra + 8 < nrows) fp8_put(p, to + (uint64_t)8 * p.N * (BF16 ? 2 : 4), u32x4a2{y[0], y[1], y[2], y[3]});
+                }
+            }
+        } else if (m < nrows) {
+#pragma unroll
+            for (int n = 0; n < NS; n += T::P) {
+                const int col = nw0 + 16 * n + T::kCols * fg;
+                float v[T::kCols];
+#pragma unroll
+                for (int c = 0; c < T::kCols; ++c) v[c] = value(n, c);
+                if (col < p.N) fp8_store<BF16, T::kCols>(p, row0 + m, col, v);
+            }
         }
     }
 }
@@ -634,6 +666,15 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     p.NB = (p.N + kFp8Block - 1) / kFp8Block;
     // Workgroups of rows x cols tiles (grouped: at most).
     auto wgs = [&](int rows, int cols) { return fp8_max_tiles(p, rows) * ((p.N + cols - 1) / cols); };
+    // Results past the caches where they are larger than an L2 (4 MB; one matrix, whose weights stay in the caches: than
+    // eight) and their rows whole lines, us without / with: 256 experts of 1024 x 2048, 8192 rows 96 / 88, 32768 141 /
+    // 132, f32 188 / 185, 1688 rows of 2816 x 704 f32 56 / 53, 8192 x 4096 x 4096 125 / 121, f32 220 / 216; 64 rows an
+    // expert (1 MB) 69 / 72.  Rows that share lines: bf16 of experts 8192 x 1000 96 / 91, 32768 139 / 137, but f32
+    // 185 / 190 and one matrix 8192 x 4001 79 / 91.  (What reads them next is no slower.)
+    const int elem = bf16 ? 2 : 4;
+    const bool whole_lines = p.N * elem % 128 == 0 && (uintptr_t)p.y % 128 == 0;
+    p.stream_out = (int64_t)p.R * p.N * elem > (p.offsets ? 4 << 20 : 32 << 20) &&
+                   (whole_lines || (p.offsets && bf16 && p.R / p.E <= 256));
     // A grid of at most two workgroups per CU that streams its operands once: latency.
     if (wgs(p.offsets ? 16 : 32, 16) <= 2 * kFp8Cus)
         return p.offsets || p.R <= 16 ? launch_stream<1, 4>(p, bf16, stream) : launch_stream<2, 2>(p, bf16, stream);
@@ -647,9 +688,6 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         return launch_tile<1, 4, 2, 2, 3>(p, bf16, stream);
     }
     const int64_t mean = p.R / p.E;
-    // bf16 results larger than an L2 past the caches where the weights go past them: 32768 rows 150 / 142 us,
-    // 4096 rows (8 MB) 89 / 85, the quantization after them no slower; 512 rows (1 MB) 69 / 72; f32 197 / 201.
-    p.stream_out = bf16 && mean <= 256 && (int64_t)p.R * p.N * 2 > (4 << 20);
     // By the rows an expert has on average: the tile that holds most experts' rows with few rows to spare.  Four
     // layers' weights in turn, us with 256x256 / 160x128 / 128x256 / 128x128 / 64x128; 256 experts of 1024 x 2048, bf16:
     // 32 rows 106 / 97 / 92 / 94 / 88, 64 rows 112 / 109 / 100 / 106 / 122, 93 rows 125 / 125 / 112 / 119, 128 rows 138 /
