@@ -31,7 +31,7 @@ __device__ __forceinline__ float fp8_act(int act, float g, float u) {
 
 template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_blocks, int cols, int act, uint8_t* q,
-                                                      float* scale) {
+                                                      float* scale, bool nt) {
     const uint32_t per_row = (uint32_t)(cols + kFp8Block - 1) / kFp8Block;
     const uint32_t id = blockIdx.x * 16u + threadIdx.x / 16u;
     if (id >= n_blocks) return;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void k_fp8_quantize(const void* x, uint32_t n_
     const float m = fp8_block_max(v);
     uint32_t o[2];
     fp8_pack8(v, m, o);
-    if (n > 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o);
+    if (n > 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o, nt);
     if ((threadIdx.x & 15) == 0) scale[id] = m / kFp8Max;
 }
 
@@ -62,9 +62,10 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
     const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
     if (blocks <= 0) return hipSuccess;
     if (blocks >= 1ll << 28) return hipErrorInvalidValue;  // (16 threads each, below 2^32 a launch)
-    const bool whole = cols % 8 == 0;
+    // nt: rows of whole lines, more than an L2 holds, past the caches (32768 x 512 x 2 f32 28.2 -> 27.4 us)
+    const bool whole = cols % 8 == 0, nt = cols % kFp8Block == 0 && rows * cols > kL2Bytes;
     const dim3 grid((unsigned)((blocks + 15) / 16));
-#define QMOE_Q8(B, V) hipLaunchKernelGGL((k_fp8_quantize<B, V>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale)
+#define QMOE_Q8(B, V) hipLaunchKernelGGL((k_fp8_quantize<B, V>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale, nt)
     if (bf16) { if (whole) QMOE_Q8(true, true); else QMOE_Q8(true, false); }
     else { if (whole) QMOE_Q8(false, true); else QMOE_Q8(false, false); }
 #undef QMOE_Q8
@@ -167,34 +168,24 @@ __device__ __forceinline__ int fp8_source_row(const Fp8Product& p, int r) {
     return s >= 0 && s < p.a_rows ? s : -1;
 }
 
-// C consecutive columns (4 or 8) of a row from column n on, up to 16 bytes at the elements'
-// alignment; those past N are left out.
-template <typename V>
-__device__ __forceinline__ void fp8_put(const Fp8Product& p, void* y, V v) {
-    if (p.stream_out) {
-        asm volatile("");  // (keeps the two stores apart: merged ones lose the hint)
-        __builtin_nontemporal_store(v, (V*)y);
-        asm volatile("");
-    } else {
-        *(V*)y = v;
-    }
-}
 template <bool BF16>
 __device__ __forceinline__ uint32_t fp8_bits(float a, float b) {  // two bf16 or one f32
     return BF16 ? f32_pack_bf16(a, b) : __builtin_bit_cast(uint32_t, a);
 }
+// C consecutive columns (4 or 8) of a row from column n on, up to 16 bytes at the elements'
+// alignment; those past N are left out.
 template <bool BF16, int C>
 __device__ __forceinline__ void fp8_store(const Fp8Product& p, int r, int n, const float (&v)[C]) {
     static_assert(C == 4 || (C == 8 && BF16), "up to 16 bytes");
     const uint64_t at = (uint64_t)r * p.N + n;
     if (n + C <= p.N) {
         if constexpr (!BF16) {
-            fp8_put(p, (float*)p.y + at, f32x4a4{v[0], v[1], v[2], v[3]});
+            put((float*)p.y + at, f32x4a4{v[0], v[1], v[2], v[3]}, p.stream_out);
         } else if constexpr (C == 4) {
-            fp8_put(p, (uint16_t*)p.y + at, u32x2a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3])});
+            put((uint16_t*)p.y + at, u32x2a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3])}, p.stream_out);
         } else {
-            fp8_put(p, (uint16_t*)p.y + at, u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
-                                                    f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])});
+            put((uint16_t*)p.y + at, u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
+                                             f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])}, p.stream_out);
         }
     } else {
 #pragma unroll
@@ -611,8 +602,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
                     }
                     const int col = nw0 + 16 * (high ? n + T::P : n) + T::kCols * fg;
                     uint8_t* const to = (uint8_t*)p.y + ((uint64_t)(row0 + ra) * p.N + col) * (BF16 ? 2 : 4);
-                    if (ra < nrows) fp8_put(p, to, u32x4a2{x[0], x[1], x[2], x[3]});
-                    if (ra + 8 < nrows) fp8_put(p, to + (uint64_t)8 * p.N * (BF16 ? 2 : 4), u32x4a2{y[0], y[1], y[2], y[3]});
+                    if (ra < nrows) put(to, u32x4a2{x[0], x[1], x[2], x[3]}, p.stream_out);
+                    if (ra + 8 < nrows) put(to + (uint64_t)8 * p.N * (BF16 ? 2 : 4), u32x4a2{y[0], y[1], y[2], y[3]}, p.stream_out);
                 }
             }
         } else if (m < nrows) {
@@ -673,7 +664,7 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     // 185 / 190 and one matrix 8192 x 4001 79 / 91.  (What reads them next is no slower.)
     const int elem = bf16 ? 2 : 4;
     const bool whole_lines = p.N * elem % 128 == 0 && (uintptr_t)p.y % 128 == 0;
-    p.stream_out = (int64_t)p.R * p.N * elem > (p.offsets ? 4 << 20 : 32 << 20) &&
+    p.stream_out = (int64_t)p.R * p.N * elem > (p.offsets ? kL2Bytes : 8 * kL2Bytes) &&
                    (whole_lines || (p.offsets && bf16 && p.R / p.E <= 256));
     // A grid of at most two workgroups per CU that streams its operands once: latency.
     if (wgs(p.offsets ? 16 : 32, 16) <= 2 * kFp8Cus)

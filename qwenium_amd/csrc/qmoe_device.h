@@ -86,12 +86,24 @@ __device__ __forceinline__ void load8(const void* x, uint64_t at, int n, float (
         for (int i = 0; i < 8; ++i) v[i] = i < n ? load1<false>(x, at + i) : 0.0f;
     }
 }
+// nt (wave-uniform): past the caches.
+template <typename V>
+__device__ __forceinline__ void put(void* y, V v, bool nt) {
+    if (nt) {
+        asm volatile("");  // (keeps the two stores apart: merged ones lose the hint)
+        __builtin_nontemporal_store(v, (V*)y);
+        asm volatile("");
+    } else {
+        *(V*)y = v;
+    }
+}
+// nt is for bf16: f32's pairs of 16 bytes share lines.
 template <bool BF16, bool WHOLE>
-__device__ __forceinline__ void store8(void* y, uint64_t at, int n, const float (&v)[8]) {
+__device__ __forceinline__ void store8(void* y, uint64_t at, int n, const float (&v)[8], bool nt = false) {
     if (WHOLE || n >= 8) {
         if constexpr (BF16) {
-            *(u32x4a2*)((uint16_t*)y + at) = u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]),
-                                                     f32_pack_bf16(v[4], v[5]), f32_pack_bf16(v[6], v[7])};
+            put((uint16_t*)y + at, u32x4a2{f32_pack_bf16(v[0], v[1]), f32_pack_bf16(v[2], v[3]), f32_pack_bf16(v[4], v[5]),
+                                           f32_pack_bf16(v[6], v[7])}, nt);
         } else {
             *(f32x4a4*)((float*)y + at) = f32x4a4{v[0], v[1], v[2], v[3]};
             *(f32x4a4*)((float*)y + at + 4) = f32x4a4{v[4], v[5], v[6], v[7]};
@@ -103,9 +115,9 @@ __device__ __forceinline__ void store8(void* y, uint64_t at, int n, const float 
     }
 }
 // 8 packed e4m3 values, of which n exist.
-__device__ __forceinline__ void store8_fp8(uint8_t* q, int n, const uint32_t (&o)[2]) {
+__device__ __forceinline__ void store8_fp8(uint8_t* q, int n, const uint32_t (&o)[2], bool nt) {
     if (n >= 8) {
-        *(u32x2a1*)q = u32x2a1{o[0], o[1]};
+        put(q, u32x2a1{o[0], o[1]}, nt);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)

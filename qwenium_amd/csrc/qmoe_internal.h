@@ -51,6 +51,8 @@ constexpr int kGateSilu = 2;
 // y[R][N] = rows of a (e4m3 [a_rows][K], scales [a_rows][KB]) times w (e4m3 [E][N][K],
 // scales [E][NB][KB]).  offsets null: one matrix; else row r belongs to the expert with
 // offsets[e] <= r < offsets[e + 1].  rows null: row r of a, else row rows[r].
+constexpr int64_t kL2Bytes = 4 << 20;  // of one XCD; the device has 8
+
 struct Fp8Product {
     const uint8_t* a;
     const float* sa;
@@ -72,6 +74,7 @@ struct ResidualNorm {
     float* q_scale;
     float scale, eps;
     int H, gate_act;
+    bool stream_out;  // outputs past the caches (set by the launcher)
 };
 
 struct LayerDesc {
@@ -286,7 +289,7 @@ hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H,
 hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, int n_tokens, int H, int top_k,
                                      const int32_t* total, const int32_t* place, const float* w, void* dys, float* dw,
                                      hipStream_t stream);
-hipError_t launch_residual_norm(const ResidualNorm& p, bool bf16, int n_tokens, hipStream_t stream);
+hipError_t launch_residual_norm(ResidualNorm p, bool bf16, int n_tokens, hipStream_t stream);
 // ggml's CPU fp16 gelu table (65536 entries): host copy, and the current device's copy.
 void gelu_table_host(uint16_t* out);
 hipError_t gelu_table_device(const uint16_t** out);

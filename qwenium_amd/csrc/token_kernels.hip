@@ -200,7 +200,6 @@ static void row_grid(int n_tokens, int64_t pieces, dim3& grid, dim3& block) {
 // than these hold (8192 x 2 rows of 8 KB 40 -> 31 us).
 // ---------------------------------------------------------------------------
 typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));
-constexpr int64_t kStreamBytes = 32 << 20;  // the L2s of 8 XCDs
 template <typename V, bool NT>
 __global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int bytes, int top_k, int R, const int32_t* total,
                                                        const int32_t* place, uint8_t* y) {
@@ -231,7 +230,7 @@ hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_col
     dim3 grid, block;
     row_grid(n_tokens, bytes >= 16 ? (bytes + 15) / 16 : bytes, grid, block);
     if (grid.y > 65535) return hipErrorInvalidValue;
-    const bool stream_out = (int64_t)n_tokens * top_k * bytes > kStreamBytes;
+    const bool stream_out = (int64_t)n_tokens * top_k * bytes > 8 * kL2Bytes;
 #define QMOE_GATHER(...)                                                                                               \
     hipLaunchKernelGGL((k_gather_tokens<__VA_ARGS__>), grid, block, 0, stream, (const uint8_t*)x, bytes, top_k,        \
                        n_tokens * top_k, total, place, (uint8_t*)y)
@@ -445,7 +444,7 @@ hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, 
                                      hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
     const int C = bf16 ? 8 : 4;
-    const bool whole = H % C == 0, stream_out = (int64_t)n_tokens * top_k * H * (16 / C) > kStreamBytes;
+    const bool whole = H % C == 0, stream_out = (int64_t)n_tokens * top_k * H * (16 / C) > 8 * kL2Bytes;
     const int64_t pieces = ((int64_t)H + C - 1) / C;
     const dim3 grid(n_tokens), block((unsigned)(pieces < 1024 ? (pieces + 63) / 64 * 64 : 1024));
 #define QMOE_BWD(...)                                                                                                  \
