@@ -356,7 +356,8 @@ enum qmoe_fp8_act {
 /* q[n_rows][n_cols] (e4m3) and scale[n_rows][ceil(n_cols/128)] of v: x itself,
  * or the activation of x's two halves (x is then [n_rows][2 n_cols], gate columns
  * first).  Per block of 128 columns (the last may be shorter) m = the largest |v|,
- * at least 1e-30: scale = m / 448, q = e4m3(v * 448 / m) rounded once, ties to even.  A
+ * at least 1e-30: scale = m / 448, q = e4m3(v * 448 / m) of the exact v and m rounded once, ties to
+ * even (of an activation to 64 bits).  A
  * block with a NaN has a NaN scale; one with an infinity an infinite scale.  Fewer than
  * 2^28 blocks. */
 int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_cols, int32_t act,

@@ -175,10 +175,10 @@ __device__ __forceinline__ float fp8_quotient(float v, float inv, float m) {
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-// e4m3 of the exact v * 448 / m, rounded once.  Quotients a little (2^-22 of them) above and
-// below mostly round to the same numbers, and then the exact ones do.
-__device__ __forceinline__ void fp8_pack8(const float (&v)[8], float m, uint32_t (&o)[2]) {
-    const float inv = kFp8Max / m, up = inv * (1.0f + 0x1p-22f), down = inv * (1.0f - 0x1p-22f);
+// o = e4m3 of v * 448 / m; true if quotients near (relative) above and below round to the same
+// numbers, as they mostly do: then the exact ones do.
+__device__ __forceinline__ bool fp8_pack8_near(const float (&v)[8], float m, float near, uint32_t (&o)[2]) {
+    const float inv = kFp8Max / m, up = inv * (1.0f + near), down = inv * (1.0f - near);
     uint32_t other = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -186,7 +186,12 @@ __device__ __forceinline__ void fp8_pack8(const float (&v)[8], float m, uint32_t
         o[h] = fp8_pack4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
         other |= o[h] ^ fp8_pack4(x[0] * down, x[1] * down, x[2] * down, x[3] * down);
     }
-    if (other == 0) return;
+    return other == 0;
+}
+// e4m3 of the exact v * 448 / m, rounded once.
+__device__ __forceinline__ void fp8_pack8(const float (&v)[8], float m, uint32_t (&o)[2]) {
+    if (fp8_pack8_near(v, m, 0x1p-22f, o)) return;
+    const float inv = kFp8Max / m;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         o[h] = fp8_pack4(fp8_quotient(h ? v[4] : v[0], inv, m), fp8_quotient(h ? v[5] : v[1], inv, m),

@@ -352,6 +352,26 @@ def test_quantize_activation(gpu, R, C, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+@pytest.mark.parametrize("R,C", [(600, 1024), (700, 333), (3, 70001)])
+def test_quantize_activation_rounds_once(gpu, R, C, act, dtype):
+    """q is the 64-bit formula's nearest e4m3, unless its quotient is the middle of two to within 64 bits' own error
+    (some 20 roundings of 2^-53, and those that gelu's z multiplies by |z| <= 60: 1e-13)."""
+    x = (2 * randn(gen(R * C), R, 2 * C)).to(dtype)
+    q, _ = qa.fp8_quantize(x.to(gpu), act=act)
+    g, u = x.double()[:, :C], x.double()[:, C:]
+    z = g if act == "swiglu" else 2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    v = torch.nn.functional.pad(u * g * torch.sigmoid(z), (0, -C % 128)).view(R, -1, 128)
+    p = (v / (v.abs().amax(2, keepdim=True).clamp_min(1e-30) / 448)).view(R, -1)[:, :C]
+    step = torch.exp2(torch.floor(torch.log2(p.abs().clamp_min(2.0 ** -6))) - 3)
+    want, got = torch.round(p / step) * step, q.cpu().double()
+    off = (got - want).abs()
+    middle = (p - (got + want) / 2).abs() <= 1e-13 * p.abs()
+    assert ((off == 0) | ((off <= step) & middle)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["swiglu", "geglu"])
 def test_quantize_activation_non_finite(gpu, act):
     """An infinite product gives its block an infinite scale, NaN a NaN one; a far negative gate gives zeros."""
