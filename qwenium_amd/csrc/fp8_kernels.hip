@@ -59,7 +59,7 @@ __device__ __forceinline__ void fp8_act_block(const void* x, uint32_t row, int c
     m = __builtin_fmax(m, __builtin_fmax(__builtin_fabs(v[0]), __builtin_fabs(v[1])));
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = __builtin_fmax(m, __shfl_xor(m, o, 64));
-    m /= kFp8Max;
+    m *= 1.0 / kFp8Max;
     const uint32_t o = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f32_odd(v[0] / m), f32_odd(v[1] / m), 0, false);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
