@@ -364,9 +364,8 @@ int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_c
                       uint8_t* q, float* scale, void* hip_stream);
 
 /* y[r][j] = sum_b a_scale[s][b] w_scale[e][j/128][b] sum_{i in block b} a[s][i] w[e][j][i]
- * (y_type f32 or bf16), sums in f32.  (For bf16 results and many rows the sums of 8
- * products within a block may drop what is below 2^-13 of the largest of them: that
- * is what the e4m3 matrix instructions keep, far below the bf16 rounding.)
+ * (y_type f32 or bf16): exact products, sums in f32, one rounding to y_type, whatever
+ * the number of rows.
  *   a [a_rows][k] e4m3, a_scale [a_rows][ceil(k/128)];
  *   w [n_experts][n][k] e4m3, w_scale [n_experts][ceil(n/128)][ceil(k/128)];
  *   offsets NULL: n_experts is 1 and every row uses the one matrix; else

@@ -128,27 +128,23 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // ---------------------------------------------------------------------------
 // Products:  y[r][n] = sum_b sa[r][b] sw[n / 128][b] sum_{k in b} a[r][k] w[n][k].
 // A block's 128 products start from zero and their sum is scaled into the f32
-// accumulators (one fma per output and block: the e4m3 MFMA's 32 cycles per 16x16x128
-// cover its 4 fmas).  Two matrix instructions can make the block's sum:
-//   f16: the operands converted to f16, which holds every e4m3 value, and
-//     v_mfma_f32_16x16x32_f16: exact products, sums with f32's 24 bits.  For f32
-//     results, and wherever memory bounds the product.
-//   e4m3: v_mfma_f32_16x16x128_f8f6f4, twice the rate, no conversions.  It aligns the
-//     products of each group of 8 columns to the largest, P, before it adds them:
-//     beside P = 2^16 a product of 2^3 counts and one of 2^2 is lost (measured; between
-//     groups all 24 bits are kept), so a group is off by less than 7 2^-13 P.  Measured
-//     2-norm error 1.5e-5 (normal values) to 7e-5 (few large ones among small) of the
-//     result: for bf16 results of the tiles, whose own rounding is 1.7e-3.
+// accumulators (one fma per output and block).  The operands are converted to f16, which
+// holds every e4m3 value, for v_mfma_f32_16x16x32_f16: exact products, sums with f32's 24
+// bits.  The e4m3 instructions are not used: they align the products of each group of 8
+// columns to the largest, P, before they add them, and drop what lies below 2^-13 P
+// (measured, 16x16x128_f8f6f4 and 16x16x32_fp8_fp8 alike: beside P = 2^16 a product of
+// 2^3 counts and one of 2^2 is lost), so that a sum whose large terms cancel is lost
+// whole.  16x16x128_f8f6f4 has 3.4 times the f16 rate (8192 x 4096 x 4096 took 125 us by
+// it); 16x16x32_fp8_fp8 has the f16 rate.
 // The weights are the MFMA's rows and the activations its columns: a lane then
 // holds four consecutive n of one row r, whose scale is one value per lane, and
 // stores them together.  (Both operands take the same permutation of a block's
 // columns, which leaves its sum as it is: lane group g reads 16-byte pieces g and
 // g + 4.)
-//   Where the time goes (us): 8192 x 4096 x 4096 bf16 121 (2.3 PFLOP/s; 275 GFLOP take
-// 93-104 in a library e4m3 product without block scales): the matrix instructions alone
-// 73, with the fmas of the scales 94, with the reads of LDS 103, the rest the loads to
-// it and the stores; f32 216 (1.3, as a library bf16 product); 256 experts of 1024 x 2048: 80 rows 25 (147 MB: 5.8 TB/s), 4096 rows 85
-// (6.3 TB/s), 32768 rows 131-136 (613 MB: 4.5-4.7 TB/s).
+//   Where the time goes (us): 8192 x 4096 x 4096 208-232 (1.2-1.3 PFLOP/s, the rate of a
+// library's bf16 product and of the f16 instruction in registers alone, 1.18), f32 results
+// 218-236; 256 experts of 1024 x 2048: 80 rows 27 (147 MB: 5.4 TB/s), 4096 rows 89 (6.0
+// TB/s), 32768 rows 185-200 (137 GFLOP: 0.7 PFLOP/s beside 613 MB).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -524,7 +520,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
             const float ws = ws_next;
             ws_next = scalar_load(sw + (b + 1 < KB ? b + 1 : b));
             const int after = buf + 1 == ST ? 0 : buf + 1;
-            f16x8 wf[BF16 ? 1 : NS][4];
+            f16x8 wf[NS][4];
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 if (LAST) {
@@ -532,28 +528,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
                     for (int c = 0; c < 8; ++c)
                         if (16 * (fg + (c & 4)) >= p.K - b * kFp8Block) wv[n][c] = 0;
                 }
-                if constexpr (!BF16) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) wf[n][q] = fp8_to_f16(wv[n][2 * q], wv[n][2 * q + 1]);
-                }
+                for (int q = 0; q < 4; ++q) wf[n][q] = fp8_to_f16(wv[n][2 * q], wv[n][2 * q + 1]);
             }
-            f16x8 af[BF16 ? 1 : kLate][4];
+            f16x8 af[kLate][4];
             auto convert = [&](int i, int to) {
-                if constexpr (!BF16) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) af[to][q] = fp8_to_f16(av[slot(i)][2 * q], av[slot(i)][2 * q + 1]);
-                }
+                for (int q = 0; q < 4; ++q) af[to][q] = fp8_to_f16(av[slot(i)][2 * q], av[slot(i)][2 * q + 1]);
             };
-            auto product = [&](int i, int n, int from) {
-                f32x4 t;
-                if constexpr (BF16) {
-                    t = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv[n], av[slot(i)], f32x4{}, 0, 0, 0, 0, 0, 0);
-                } else {
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][0], af[from][0], f32x4{}, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][1], af[from][1], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][2], af[from][2], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][3], af[from][3], t, 0, 0, 0);
-                }
+            auto product = [&](int n, int from) {
+                f32x4 t = {};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[n][q], af[from][q], t, 0, 0, 0);
                 return t;
             };
             auto add = [&](int i, int n, float s, f32x4 t) {
@@ -569,10 +555,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
                 convert(i, 0);
                 f32x4 t[NS];
 #pragma unroll
-                for (int n = 0; n < NS; ++n) t[n] = product(i, n, 0);
+                for (int n = 0; n < NS; ++n) t[n] = product(n, 0);
 #pragma unroll
                 for (int n = 0; n < NS; ++n) add(i, n, s, t[n]);
-                if (!BF16) __builtin_amdgcn_sched_barrier(0);  // (loads moved up from the next subtile would spill)
+                __builtin_amdgcn_sched_barrier(0);  // (loads moved up from the next subtile would spill)
             }
             if (kLate == 2) rows(MI - 1, b, buf);
             if (!LAST) {
@@ -600,7 +586,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
             for (int n = 0; n < NS; ++n) {
                 f32x4 t[kLate];
 #pragma unroll
-                for (int j = 0; j < kLate; ++j) t[j] = product(MI - kLate + j, n, j);
+                for (int j = 0; j < kLate; ++j) t[j] = product(n, j);
                 if (!LAST) weights(n, after);
 #pragma unroll
                 for (int j = 0; j < kLate; ++j) add(MI - kLate + j, n, s[j], t[j]);
@@ -724,28 +710,27 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         return p.offsets || p.R <= 16 ? launch_stream<1, 4>(p, bf16, stream) : launch_stream<2, 2>(p, bf16, stream);
     if (!p.offsets) {
         // The largest tile that gives every CU a workgroup.  Rows x 4096 x 4096, bf16, us with tiles of
-        // 256x256 / 128x256 / 64x128 / 32x128: 4096 rows 63 / 76 / 97, 2048 52 / 38 / 50 / 65, 1024 51 / 34 / 26 / 40,
-        // 256 51 / 33 / 18 / 15.
+        // 256x256 / 128x256 / 64x128 / 32x128: 4096 rows 106 / 121 / 148, 2048 97 / 62 / 76, 1024 95 / 58 / 41, 512 95 /
+        // 57 / 28, 256 94 / 56 / 27 / 21.
         if (wgs(256, 256) >= kFp8Cus) return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
         if (wgs(64, 128) >= kFp8Cus) return launch_tile<1, 4, 4, 2, 3>(p, bf16, stream);
         return launch_tile<1, 4, 2, 2, 3>(p, bf16, stream);
     }
     const int64_t mean = p.R / p.E;
-    // By the rows an expert has on average: the tile that holds most experts' rows with few rows to spare.  Four
+    // By the rows an expert has on average: the tile that holds most experts' rows with few rows to spare.  Several
     // layers' weights in turn, us with 256x256 / 160x128 / 128x256 / 128x128 / 64x128; 256 experts of 1024 x 2048, bf16:
-    // 32 rows 106 / 97 / 92 / 94 / 88, 64 rows 112 / 109 / 100 / 106 / 122, 93 rows 125 / 125 / 112 / 119, 128 rows 138 /
-    // 137 / 150 / 160, 156 rows 159 / 168 / 186 / 193, 187 rows 167 / 212 / 199 / 205; 128 of 1408 x 2816, 125 rows 138 /
-    // 130 / 145 / 149; f32: 64 rows 150 / 144 / 139 / 135 / 145, 128 rows 220 / 195 / 216 / 208; 128 of 2816 x 704, 62
-    // rows 99 / 89 / 96 / 87 / 90; through the caches 256 experts, 156 rows 261 / 235, 187 rows 266 / 300; 64 of
-    // 1536 x 1536, 281 rows, bf16 87 / 79 / 90, f32 147 / 116 / 134.
+    // 32 rows 116 / 101 / 102 / 98 / 96, 64 rows 144 / 138 / 136 / 126 / 137, 93 rows 161 / 173 / 159 / 154 / 187, 128 rows
+    // 218 / 185 / 203 / 198 / 227, 156 rows 246 / 220 / 242 / 237 / 267, 187 rows 254 / 274 / 281 / 271 / 302; f32: 64 rows
+    // 150 / 138 / 136 / 129 / 142, 128 rows 222 / 189 / 210 / 206 / 233, 187 rows 269 / 285 / 292 / 279 / 314; 128 of 1408 x
+    // 2816, 125 rows 221 / 176 / 201 / 184 / 210; 128 of 2816 x 704, 62 rows 93 / 85 / 92 / 81 / 86, f32 97 / 91 / 96 / 87 /
+    // 93; 64 of 1536 x 1536, 281 rows 131 / 105 / 121 / 114 / 134; 8 of 2048 x 2048, 2000 rows 125 / 133 / 134 / 130 / 160.
     if (mean >= 110) {
-        if (((mean > (bf16 ? 140 : 160) && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
+        if (((mean > 160 && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
             return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
         if (wgs(160, 128) >= kFp8Cus) return launch_tile<2, 2, 5, 4, 2>(p, bf16, stream);
-    } else if (mean >= 56) {
-        if (bf16 && wgs(128, 256) >= kFp8Cus) return launch_tile<2, 4, 4, 4, 3>(p, bf16, stream);
-        if (!bf16 && wgs(128, 128) >= kFp8Cus) return launch_tile<2, 2, 4, 4, 2>(p, bf16, stream);
+    } else if (mean >= 56 && wgs(128, 128) >= kFp8Cus) {
+        return launch_tile<2, 2, 4, 4, 2>(p, bf16, stream);
     }
     // Weights streamed for few rows: small tiles, many loads in flight, unless K is soon over; up to 20 rows also where
     // there would be few large tiles.  Us with 32x64 in four buffers / in three / 64x128 in three / in two: 256 experts

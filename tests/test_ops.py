@@ -527,6 +527,41 @@ def test_matmul_tile_sizes(gpu, E, R, N, K, dtype):
             assert off.max() <= 0, f"expert {e}: {off.max().item():.3e} over its tolerance"
 
 
+# experts (0: dense), rows, n, k: the kernel of few rows, then every tile
+SUMS = [(0, 3, 200, 144), (0, 40, 520, 1040), (0, 300, 520, 1024), (0, 600, 2100, 528), (0, 2050, 4100, 400), (0, 4100, 4104, 400),
+        (3, 9, 64, 272), (8, 1500, 5128, 272), (8, 2000, 1704, 272), (16, 1280, 2696, 400), (8, 900, 1000, 1040), (40, 700, 900, 656),
+        (300, 2400, 260, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E,R,N,K", SUMS)
+def test_matmul_large_products_that_cancel(gpu, E, R, N, K, dtype):
+    """Of every 8 columns two hold 448 x 448 and 448 x -448, the others whole numbers up to 3.  All products are whole
+    and those of a block of 128 add up to less than 32 x 448^2 + 96 x 9 < 2^23, so sums of 24 bits are exact in any
+    order, whatever the number of rows: y is the small numbers' sum, rounded to its type once."""
+    g = gen(R + N + K)
+
+    def small(*shape):
+        return torch.randint(-3, 4, shape, generator=g).float()
+
+    a, w = small(R, K), small(max(E, 1), N, K)
+    pair = torch.argsort(torch.rand(K // 8, 8, generator=g), 1)[:, :2] + 8 * torch.arange(K // 8)[:, None]
+    a[:, pair] = 0
+    w[:, :, pair] = 0
+    bounds = torch.linspace(0, R, max(E, 1) + 1).int()
+    want = torch.cat([a[bounds[e]:bounds[e + 1]].to(gpu) @ w[e].to(gpu).T for e in range(max(E, 1))]).to(dtype)
+    a[:, pair] = 448.0
+    w[:, :, pair[:, 0]], w[:, :, pair[:, 1]] = 448.0, -448.0
+    s, sw = torch.ones(R, blocks(K), device=gpu), torch.ones(max(E, 1), blocks(N), blocks(K), device=gpu)
+    a, w = a.to(gpu).to(FP8), w.to(gpu).to(FP8)
+    if E:
+        y = qa.fp8_matmul(a, s, w, sw, offsets=bounds.to(gpu), out_dtype=dtype)
+    else:
+        y = qa.fp8_matmul(a, s, w[0], sw[0], out_dtype=dtype)
+    assert torch.equal(y, want)
+
+
 @pytest.mark.gpu
 def test_matmul_beyond_32_bit_offsets(gpu):
     """Rows, experts and outputs whose byte offsets pass 2^32."""
