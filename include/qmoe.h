@@ -357,7 +357,7 @@ enum qmoe_fp8_act {
  * or the activation of x's two halves (x is then [n_rows][2 n_cols], gate columns
  * first).  Per block of 128 columns (the last may be shorter) m = the largest |v|,
  * at least 1e-30: scale = m / 448, q = e4m3(v * 448 / m) of the exact v and m rounded once, ties to
- * even (of an activation to 64 bits).  A
+ * even (of an activation to 64 bits; its scale from m in f32, to v's own roundings).  A
  * block with a NaN has a NaN scale; one with an infinity an infinite scale.  Fewer than
  * 2^28 blocks. */
 int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_cols, int32_t act,

@@ -20,24 +20,29 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // 448 is e4m3's largest value.  kFp8Tiny keeps 448 / m finite; a block of zeros has
 // zeros.
 // q of an activation is the formula's number rounded once too: where f32's errors in v and m
-// could put a quotient on the other side of the middle of two e4m3 numbers (a block in 700),
-// the block is made again in f64.
+// could put a quotient on the other side of the middle of two e4m3 numbers (a block in some
+// 300), the block is made again in f64.  Its scale is m / 448 of the f32 m.
 // 16 lanes take a block, 8 columns each (one or two 16-byte loads), so a wave
 // covers 512 columns; no LDS, no barrier.  Bound by memory: 4096 x 2048 f32 (42 MB) 8.2
 // us, 5.1 TB/s (0.5 of it for the exact quotients); 32768 x 512 SwiGLU of bf16 (84 MB)
-// 18.5-19.5 us, 4.4 TB/s, level with its arithmetic (2 more with expf; 0.5 of it for the
-// blocks in f64, whose registers are kept within eight waves a SIMD).
+// 18.5-19.9 us, 4.4 TB/s, level with its arithmetic (2 more with expf; 0.5 of it for the
+// blocks in f64, whose registers are kept within eight waves a SIMD); GeGLU 22.6-22.9, of
+// gates N(0, 4) 26.9, its values' own error bounds 0.8-1 of it.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float fp8_act(int act, float g, float u) {
-    // gelu's tanh form is g sigmoid(2 z) with z = sqrt(2/pi) (g + 0.044715 g^3)
-    return sigmoid_product(g, act == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g), u);
+// v = g sigmoid(z) u and a bound of its relative error.  sigmoid_product is off by up to 5 2^-24 (the hardware's 2^t 2, its
+// remainder 1, the quotient 1/2, the product 1).  SwiGLU's z is g; gelu's tanh form has z = 2 sqrt(2/pi) (g + 0.044715 g^3),
+// which carries up to 6 2^-24 of itself (its constants, two products of the cubic part, the sum, the last product), and
+// these count |z| e^-z / (1 + e^-z) times in v: |z| times below zero, at most 0.28 times above.
+constexpr float kU32 = 0x1p-24f;  // half a step of f32
+template <int ACT>
+__device__ __forceinline__ float fp8_act(float g, float u, float& off) {
+    const float z = ACT == kFp8ActSwiglu ? g : 1.5957691216057308f * fmaf(0.044715f * g * g, g, g);
+    off = ACT == kFp8ActSwiglu ? 5 * kU32 : fmaf(-6 * kU32, __builtin_fminf(__builtin_fmaxf(z, -1e6f), 0.0f), 7 * kU32);
+    return sigmoid_product(g, z, u);
 }
-
-// The relative error of fp8_act's values and of their maximum together, with room: the hardware's 2^t
-// and four roundings each (2^-21.4); gelu's z adds its own roundings, |z| 2^-22 (for |z| up to 6).
-__device__ __forceinline__ float fp8_act_error(int act) { return act == kFp8ActSwiglu ? 0x1p-21f : 0x1p-18f; }
-__device__ __forceinline__ double fp8_act_exact(int act, double g, double u) {
-    const double z = act == kFp8ActSwiglu ? g : 1.5957691216057308 * (g + 0.044715 * g * g * g);
+template <int ACT>
+__device__ __forceinline__ double fp8_act_exact(double g, double u) {
+    const double z = ACT == kFp8ActSwiglu ? g : 1.5957691216057308 * (g + 0.044715 * g * g * g);
     return u * g * (1.0 / (1.0 + exp(-z)));
 }
 // f64 to f32 for one more rounding to a type of fewer bits: cut off, the last bit set if anything was.
@@ -48,14 +53,14 @@ __device__ __forceinline__ float f32_odd(double v) {
     return __builtin_bit_cast(float, b);
 }
 // Block id's q in f64, by the whole wave: two columns a lane.
-template <bool BF16>
-__device__ __forceinline__ void fp8_act_block(const void* x, uint32_t row, int c0, int cols, int act, uint8_t* q) {
+template <bool BF16, int ACT>
+__device__ __forceinline__ void fp8_act_block(const void* x, uint32_t row, int c0, int cols, uint8_t* q) {
     const int c = c0 + 2 * ((int)threadIdx.x & 63);
     const uint64_t at = (uint64_t)row * 2 * cols + c;
     double v[2] = {}, m = kFp8Tiny;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        if (c + i < cols) v[i] = fp8_act_exact(act, load1<BF16>(x, at + i), load1<BF16>(x, at + cols + i));
+        if (c + i < cols) v[i] = fp8_act_exact<ACT>(load1<BF16>(x, at + i), load1<BF16>(x, at + cols + i));
     m = __builtin_fmax(m, __builtin_fmax(__builtin_fabs(v[0]), __builtin_fabs(v[1])));
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = __builtin_fmax(m, __shfl_xor(m, o, 64));
@@ -66,39 +71,49 @@ __device__ __forceinline__ void fp8_act_block(const void* x, uint32_t row, int c
         if (c + i < cols) q[(uint64_t)row * cols + c + i] = (uint8_t)(o >> (8 * i));
 }
 
-template <bool BF16, bool WHOLE, bool ACT>
-__global__ __launch_bounds__(256, 8) void k_fp8_quantize(const void* x, uint32_t n_blocks, int cols, int act, uint8_t* q,
-                                                      float* scale, bool nt) {
+template <bool BF16, bool WHOLE, int ACT>
+__global__ __launch_bounds__(256, 8) void k_fp8_quantize(const void* x, uint32_t n_blocks, int cols, uint8_t* q, float* scale,
+                                                      bool nt) {
     const uint32_t per_row = (uint32_t)(cols + kFp8Block - 1) / kFp8Block;
     const uint32_t id = blockIdx.x * 16u + threadIdx.x / 16u;
     const uint32_t row = id / per_row;
     const int c0 = (int)(id - row * per_row) * kFp8Block + 8 * ((int)threadIdx.x & 15);
     const int n = id < n_blocks ? cols - c0 : 0;  // columns from c0 on: none or some of this lane's 8 may exist
-    float v[8] = {};
+    float v[8] = {}, off[8] = {};
     if (n > 0) {
-        if constexpr (!ACT) {
+        if constexpr (ACT == kFp8ActNone) {
             load8<BF16, WHOLE>(x, (uint64_t)row * cols + c0, n, v);
         } else {
             float u[8];
             load8<BF16, WHOLE>(x, (uint64_t)row * 2 * cols + c0, n, v);
             load8<BF16, WHOLE>(x, (uint64_t)row * 2 * cols + cols + c0, n, u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fp8_act(act, v[i], u[i]);
+            for (int i = 0; i < 8; ++i) v[i] = fp8_act<ACT>(v[i], u[i], off[i]);
         }
     }
     const float m = fp8_block_max(v);
     uint32_t o[2];
-    if constexpr (!ACT) {
+    if constexpr (ACT == kFp8ActNone) {
         fp8_pack8(v, m, o);
         if (n > 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o, nt);
     } else {
-        uint64_t open = __ballot(!fp8_pack8_near(v, m, fp8_act_error(act), o));
+        // the quotients' own roundings (448 / m, its two neighbours, the two products), and m's error: the largest of
+        // |v| (1 + off) lies as far above the exact maximum's least value as that above m's
+        float near = 12 * kU32;
+        if constexpr (ACT == kFp8ActGeglu) {
+            float above[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) above[i] = fmaf(__builtin_fabsf(v[i]), off[i], __builtin_fabsf(v[i]));
+            const float top = fp8_block_max(above);
+            if (m < __builtin_huge_valf()) near = fmaf(1.0f / m, top - m, 7 * kU32);
+        }
+        uint64_t open = __ballot(!fp8_pack8_near(v, off, m, near, o));
         if (n > 0 && (open >> (threadIdx.x & 48) & 0xffff) == 0) store8_fp8(q + (uint64_t)row * cols + c0, n, o, nt);
         while (open) {
             const int first = __builtin_ctzll(open) & 48;  // the block's first lane
             open &= ~(0xffffull << first);
-            fp8_act_block<BF16>(x, (uint32_t)__builtin_amdgcn_readlane((int)row, first),
-                                __builtin_amdgcn_readlane(c0, first), cols, act, q);
+            fp8_act_block<BF16, ACT>(x, (uint32_t)__builtin_amdgcn_readlane((int)row, first),
+                                __builtin_amdgcn_readlane(c0, first), cols, q);
         }
     }
     if (n > 0 && (threadIdx.x & 15) == 0) scale[id] = m / kFp8Max;
@@ -112,16 +127,18 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
     // nt: rows of whole lines, more than an L2 holds, past the caches (32768 x 512 x 2 f32 28.2 -> 27.4 us)
     const bool whole = cols % 8 == 0, nt = cols % kFp8Block == 0 && rows * cols > kL2Bytes;
     const dim3 grid((unsigned)((blocks + 15) / 16));
-#define QMOE_Q8(B, V)                                                                                                  \
-    do {                                                                                                               \
-        if (act == kFp8ActNone)                                                                                        \
-            hipLaunchKernelGGL((k_fp8_quantize<B, V, false>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale, nt); \
-        else                                                                                                           \
-            hipLaunchKernelGGL((k_fp8_quantize<B, V, true>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, act, q, scale, nt); \
+#define QMOE_Q8A(B, V, A) \
+    hipLaunchKernelGGL((k_fp8_quantize<B, V, A>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, q, scale, nt)
+#define QMOE_Q8(B, V)                                              \
+    do {                                                           \
+        if (act == kFp8ActNone) QMOE_Q8A(B, V, kFp8ActNone);       \
+        else if (act == kFp8ActSwiglu) QMOE_Q8A(B, V, kFp8ActSwiglu); \
+        else QMOE_Q8A(B, V, kFp8ActGeglu);                         \
     } while (0)
     if (bf16) { if (whole) QMOE_Q8(true, true); else QMOE_Q8(true, false); }
     else { if (whole) QMOE_Q8(false, true); else QMOE_Q8(false, false); }
 #undef QMOE_Q8
+#undef QMOE_Q8A
     return hipGetLastError();
 }
 

@@ -175,22 +175,23 @@ __device__ __forceinline__ float fp8_quotient(float v, float inv, float m) {
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
 }
-// o = e4m3 of v * 448 / m; true if quotients near (relative) above and below round to the same
-// numbers, as they mostly do: then the exact ones do.
-__device__ __forceinline__ bool fp8_pack8_near(const float (&v)[8], float m, float near, uint32_t (&o)[2]) {
-    const float inv = kFp8Max / m, up = inv * (1.0f + near), down = inv * (1.0f - near);
+// o = e4m3 of v * 448 / m; true if quotients near (relative) above and below round to the same numbers, as they mostly
+// do: then the exact ones do.  off: v's own relative errors, below 1 (null: none).
+__device__ __forceinline__ bool fp8_pack8_near(const float (&v)[8], const float* off, float m, float near, uint32_t (&o)[2]) {
+    const float inv = kFp8Max / m, up = fmaf(inv, near, inv), down = fmaf(inv, -near, inv);
     uint32_t other = 0;
+    auto high = [&](int i) { return v[i] * (off ? fmaf(up, off[i], up) : up); };
+    auto low = [&](int i) { return v[i] * (off ? fmaf(down, -off[i], down) : down); };  // (a product: a zero keeps its sign)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const float* x = v + 4 * h;
-        o[h] = fp8_pack4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
-        other |= o[h] ^ fp8_pack4(x[0] * down, x[1] * down, x[2] * down, x[3] * down);
+        o[h] = fp8_pack4(high(4 * h), high(4 * h + 1), high(4 * h + 2), high(4 * h + 3));
+        other |= o[h] ^ fp8_pack4(low(4 * h), low(4 * h + 1), low(4 * h + 2), low(4 * h + 3));
     }
     return other == 0;
 }
 // e4m3 of the exact v * 448 / m, rounded once.
 __device__ __forceinline__ void fp8_pack8(const float (&v)[8], float m, uint32_t (&o)[2]) {
-    if (fp8_pack8_near(v, m, 0x1p-22f, o)) return;
+    if (fp8_pack8_near(v, nullptr, m, 0x1p-22f, o)) return;  // (three roundings: of 448 / m, its neighbour, the product)
     const float inv = kFp8Max / m;
 #pragma unroll
     for (int h = 0; h < 2; ++h)

@@ -372,6 +372,36 @@ def test_quantize_activation_rounds_once(gpu, R, C, act, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ["swiglu", "geglu"])
+@pytest.mark.parametrize("low,high", [(-9, -7), (-9, -5), (-14, -9), (-30, 4), (-1, 12)])
+def test_quantize_activation_rounds_once_far_gates(gpu, low, high, act, dtype):
+    """As above for blocks whose gates all lie between low and high: far below zero z's own roundings count |z| times in
+    the value and in the block's maximum.  (64 bits: where |v| counts beside 1e-30 / 448, z > -81, and up to
+    20 roundings of 2^-53 of it are 2e-13.)"""
+    R, C = 3001, 4096
+    g = torch.Generator(device=gpu).manual_seed(1000 - 31 * low + high)
+    x = torch.empty(R, 2 * C, device=gpu)
+    x[:, :C] = low + (high - low) * torch.rand(R, C, generator=g, device=gpu)
+    x[:, C:] = 2 * torch.randn(R, C, generator=g, device=gpu)
+    x = x.to(dtype)
+    q, s = qa.fp8_quantize(x, act=act)
+    gate, up = x.double()[:, :C], x.double()[:, C:]
+    z = gate if act == "swiglu" else 2 * math.sqrt(2 / math.pi) * (gate + 0.044715 * gate ** 3)
+    v = (up * gate * torch.sigmoid(z)).view(R, -1, 128)
+    m = v.abs().amax(2, keepdim=True).clamp_min(1e-30)
+    p = (v * 448 / m).view(R, C)
+    step = torch.exp2(torch.floor(torch.log2(p.abs().clamp_min(2.0 ** -6))) - 3)
+    want, got = torch.round(p / step) * step, q.double()
+    off = (got - want).abs()
+    middle = (p - (got + want) / 2).abs() <= 4e-13 * p.abs()
+    assert ((off == 0) | ((off <= step) & middle)).all(), f"{int(((off > 0) & ~middle).sum())} of {R * C} values"
+    # the scale: z's 6 roundings counted |z| times, 8 others, 2 of its own
+    far = 0.0 if act == "swiglu" else float(6 * z.abs().max())
+    assert ((s.double() - m[:, :, 0] / 448).abs() <= (10 + far) * U32 * m[:, :, 0] / 448).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["swiglu", "geglu"])
 def test_quantize_activation_non_finite(gpu, act):
     """An infinite product gives its block an infinite scale, NaN a NaN one; a far negative gate gives zeros."""
