@@ -358,8 +358,8 @@ enum qmoe_fp8_act {
  * first).  Per block of 128 columns (the last may be shorter) m = the largest |v|,
  * at least 1e-30: scale = m / 448, q = e4m3(v * 448 / m) of the exact v and m rounded once, ties to
  * even (of an activation to 64 bits; its scale from m in f32, to v's own roundings).  A
- * block with a NaN has a NaN scale; one with an infinity an infinite scale.  Fewer than
- * 2^28 blocks. */
+ * block with a NaN has a NaN scale; one with an infinity an infinite scale.  At most
+ * 2^28 - 16 blocks. */
 int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_cols, int32_t act,
                       uint8_t* q, float* scale, void* hip_stream);
 

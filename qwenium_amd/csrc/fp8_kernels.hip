@@ -123,7 +123,7 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
                                hipStream_t stream) {
     const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
     if (blocks <= 0) return hipSuccess;
-    if (blocks >= 1ll << 28) return hipErrorInvalidValue;  // (16 threads each, below 2^32 a launch)
+    if (blocks > (1ll << 28) - 16) return hipErrorInvalidValue;  // (16 threads each in whole workgroups of 256, below 2^32 a launch)
     // nt: rows of whole lines, more than an L2 holds, past the caches (32768 x 512 x 2 f32 28.2 -> 27.4 us)
     const bool whole = cols % 8 == 0, nt = cols % kFp8Block == 0 && rows * cols > kL2Bytes;
     const dim3 grid((unsigned)((blocks + 15) / 16));

@@ -70,8 +70,9 @@ int check_tokens(int32_t n_tokens, int32_t top_k) {
     return in_range("n_tokens * top_k", (int64_t)n_tokens * top_k, 0, 1 << 30);
 }
 
-// A launch holds below 2^32 threads; a row takes up to 1024 (16 a block of the quantization).
-constexpr int64_t kMaxRowLaunch = (1 << 22) - 1, kMaxBlocks = (1 << 28) - 1;
+// A launch holds below 2^32 threads; a row takes up to 1024 (16 a block of the quantization, whose last workgroup of 16
+// blocks is a whole one).
+constexpr int64_t kMaxRowLaunch = (1 << 22) - 1, kMaxBlocks = (1 << 28) - 16;
 
 #define QMOE_TRY(expr)                   \
     do {                                 \

@@ -130,6 +130,15 @@ def test_quantize_refusals(kw, code, needle):
     assert needle in _lib.last_error() and "expected" in _lib.last_error()
 
 
+def test_quantize_blocks_of_one_launch():
+    """16 threads a block in whole workgroups of 16 blocks, below 2^32 threads: up to 2^28 - 16 blocks."""
+    for R, C in ((2 ** 28 - 15, 1), (2 ** 28 - 1, 128), (2 ** 27 - 7, 129)):
+        assert rc_quantize(R=R, C=C, x=None) == QMOE_ERR_VALUE
+        assert f"ceil(n_cols/128) expected 0..{2 ** 28 - 16}" in _lib.last_error()
+    for R, C in ((2 ** 28 - 16, 1), (2 ** 27 - 8, 129)):  # (the next check's answer)
+        assert rc_quantize(R=R, C=C, x=None) == QMOE_ERR_NULL
+
+
 def test_no_rows_is_a_no_op_without_gpu():
     L = _lib.lib()
     assert rc_quantize(R=0, x=None, q=None, s=None) == QMOE_OK
