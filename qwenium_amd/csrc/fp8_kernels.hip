@@ -687,7 +687,7 @@ static int64_t fp8_max_tiles(const Fp8Product& p, int tile) {
 template <int MT, int U>
 static hipError_t launch_stream(const Fp8Product& p, bool bf16, hipStream_t stream) {
     const int64_t blocks = fp8_max_tiles(p, 16 * MT) * ((p.N + 15) / 16);
-    if (blocks >= 1ll << 24) return hipErrorInvalidValue;  // (below 2^32 threads)
+    if (blocks >= 1ll << 24) return hipErrorInvalidConfiguration;  // (below 2^32 threads)
     if (bf16) hipLaunchKernelGGL((k_fp8_stream<MT, U, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((k_fp8_stream<MT, U, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     return hipGetLastError();
@@ -698,7 +698,7 @@ static hipError_t launch_tile_as(const Fp8Product& p, hipStream_t stream) {
     using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
     const int64_t tiles = fp8_max_tiles(p, T::kBM), nt = (p.N + T::kBN - 1) / T::kBN;
     const int64_t blocks = p.offsets ? (tiles + 7) / 8 * 8 * nt : (tiles * nt + 7) / 8 * 8;
-    if (blocks * (64 * T::kWaves) >= 1ll << 32) return hipErrorInvalidValue;
+    if (blocks * (64 * T::kWaves) >= 1ll << 32) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((k_fp8_tile<WM, WN, MS, NS, ST, BF16>), dim3((unsigned)blocks), dim3(64 * T::kWaves), T::kLds, stream, p);
     return hipGetLastError();
 }

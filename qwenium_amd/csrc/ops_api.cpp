@@ -148,7 +148,10 @@ int qmoe_fp8_matmul(const uint8_t* a, const float* a_scale, int32_t a_rows, cons
     p.N = n;
     p.K = k;
     p.R = n_rows;
-    return done(qmoe::launch_fp8_matmul(p, y_type == QMOE_TYPE_BF16, (hipStream_t)hip_stream), "fp8_matmul kernel");
+    const hipError_t err = qmoe::launch_fp8_matmul(p, y_type == QMOE_TYPE_BF16, (hipStream_t)hip_stream);
+    if (err == hipErrorInvalidConfiguration)
+        return bad_value("n_rows x n", "fewer than 2^32 threads in tiles of its rows and columns", str(n_rows) + " x " + str(n));
+    return done(err, "fp8_matmul kernel");
 }
 
 int qmoe_sort_tokens(const int32_t* topk_idx, int32_t n_tokens, int32_t top_k, int32_t n_experts, int32_t* offsets,

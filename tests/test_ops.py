@@ -173,6 +173,13 @@ def test_matmul_refusals(kw, code, needle):
     assert needle in _lib.last_error()
 
 
+def test_matmul_larger_than_a_launch():
+    """1024 experts with a row each and 2^23 columns are 2^26 workgroups or more: refused by name, before the launch."""
+    a, b, c, d, e, f = (FAKE + (i << 40) for i in range(6))
+    assert rc_matmul(a=a, sa=b, A=1024, w=c, sw=d, E=1024, n=2 ** 23, k=16, offsets=e, R=1024, y=f) == QMOE_ERR_VALUE
+    assert "n_rows x n expected fewer than 2^32 threads" in _lib.last_error() and "1024 x 8388608" in _lib.last_error()
+
+
 def test_token_refusals():
     L = _lib.lib()
     a, b, c, d, e = (FAKE + i * MIB for i in range(5))
