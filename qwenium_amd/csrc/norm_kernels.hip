@@ -15,8 +15,8 @@ namespace qmoe {
 // that the row stays in registers between the loads and the stores: each operand
 // is read once, and 16 neighbouring threads hold a block of 128 columns.  The sums
 // of squares are f64 of the f32 squares (a thread's in turn, the tree over a wave's
-// lanes, the waves in turn).  h and q come from the f32 x', not from its rounding
-// to the rows' type.  Bound by memory: 4096 x 2816 bf16 with both norms, gate and a
+// lanes, the waves in turn), as rms_norm's but for rows whose squares leave f32's range.
+// h and q come from the f32 x', not from its rounding to the rows' type.  Bound by memory: 4096 x 2816 bf16 with both norms, gate and a
 // scale per column (115 MB) 24.4 us, 4.7 TB/s (26.1 with its outputs through
 // the caches, 28.0 with expf and a division too; inputs out of memory 29.3); f32 5.3 TB/s.
 // ---------------------------------------------------------------------------
@@ -29,9 +29,34 @@ __device__ __forceinline__ double block_sum_f64(double v, double* s) {
     return t;
 }
 
+// The row's r = 1 / sqrt(mean(v^2) + eps).  Where squares may leave f32 (the largest above 2^126, or the mean with eps below
+// 2^-110, beside which a square's error below 2^-126, 2^-150, would count), v is scaled by a power of two and r is that
+// of the scaled row: v r is as it was.
+template <int NP>
+__device__ __forceinline__ float norm_row(float (&v)[NP][8], int H, float eps, double* s_sum) {
+    auto ssq = [&](double* sums) {
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) s += (double)(v[i][c] * v[i][c]);  // (columns past H are zeros)
+        return block_sum_f64(s, sums);
+    };
+    float r = rms_scale_from_ssq(ssq(s_sum), H, eps);
+    if (!(r >= 0x1p-63f && r <= 0x1p55f)) {
+        const float by = r > 0x1p55f ? 0x1p100f : 0x1p-66f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[i][c] *= by;
+        r = rms_scale_from_ssq(ssq(s_sum + 16), H, eps * by * by);
+    }
+    return r;
+}
+
 template <bool BF16, bool WHOLE, int NP>
 __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
-    __shared__ double s_sum[2][16];
+    __shared__ double s_sum[4][16];
     const uint64_t row = (uint64_t)blockIdx.x * p.H;
     const int H = p.H;
     float v[NP][8] = {}, u[NP][8] = {}, g[NP][8] = {};
@@ -47,14 +72,7 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
     }
     if (p.y) {
         float post = 1.0f;
-        if (p.post_w) {
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) s += (double)(u[i][c] * u[i][c]);
-            post = rms_scale_from_ssq(block_sum_f64(s, s_sum[0]), H, p.eps);
-        }
+        if (p.post_w) post = norm_row(u, H, p.eps, s_sum[0]);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             if (n[i] <= 0) continue;
@@ -81,11 +99,6 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
             store8<BF16, WHOLE>(p.x_out, row + c0[i], n[i], v[i], p.stream_out);
         }
     }
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) s += (double)(v[i][c] * v[i][c]);  // (columns past H are zeros)
     float w[NP][8];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -93,7 +106,7 @@ __global__ __launch_bounds__(1024) void k_residual_norm(ResidualNorm p) {
         for (int c = 0; c < 8; ++c) w[i][c] = 1.0f;
         if (p.w && n[i] > 0) load8<false, WHOLE>(p.w, c0[i], n[i], w[i]);
     }
-    const float r = rms_scale_from_ssq(block_sum_f64(s, s_sum[1]), H, p.eps);
+    const float r = norm_row(v, H, p.eps, s_sum[2]);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
 #pragma unroll

@@ -902,6 +902,36 @@ def test_residual_norm(gpu, T, H, post, gate, vector, quantize, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mag,eps", [(1e25, 1e-6), (3e38, 1e-6), (2e19, 0.0), (1e-25, 0.0), (2e-38, 0.0), (1e-17, 1e-38),
+                                     (1e-25, 1e-6), (1e-20, 1e-38), (1.0, 3e38)])
+@pytest.mark.parametrize("T,H", [(3, 1), (5, 200), (4, 2816), (2, 16384)])
+def test_residual_norm_magnitudes(gpu, T, H, mag, eps, dtype):
+    """Rows whose squares leave f32's range, in the residual rows and before the norm after the block; a row of each beside
+    ordinary ones, which keep their bits."""
+    g = gen(T + H)
+    big = ((2 * torch.rand(T, H, generator=g) - 1) * mag).to(dtype)
+    big[:, 0] = mag
+    one, w = randn(g, T, H).to(dtype), 1 + 0.2 * randn(g, H)
+    eps = float(np.float32(eps))  # what the call takes
+    u = 0.0 if dtype == torch.float32 else U[dtype]
+    rows = one.clone()
+    rows[::2] = big[::2]
+    n = qa.residual_norm(rows.to(gpu), None, w.to(gpu), eps, quantize=True)
+    _, want, _, eh = plain_norm(rows, None, w, eps)
+    tiny = 2.0 ** -149  # (f32's and bf16's smallest steps: 2^-149, 2^-133)
+    near(n.h, want, eh + (U32 + u * (1 + 2.0 ** -8)) * want.abs() + (tiny if dtype == torch.float32 else 2.0 ** -133), "h")
+    assert torch.equal(n.h[1::2].cpu(), qa.residual_norm(one.to(gpu), None, w.to(gpu), eps).h[1::2].cpu())
+    y = one.clone()
+    y[::2] = big[::2]
+    n = qa.residual_norm(one.to(gpu), y.to(gpu), w.to(gpu), eps, post_w=w.to(gpu), scale=0.5)
+    yd = y.double()
+    v = 0.5 * yd / torch.sqrt((yd * yd).mean(1, keepdim=True) + eps) * w.double()
+    want = one.double() + v
+    near(n.x, want, 12 * U32 * v.abs() + (U32 + u * (1 + 2.0 ** -8)) * want.abs() + tiny, "x")
+
+
+@pytest.mark.gpu
 def test_residual_norm_alone_and_in_place(gpu):
     g = gen(2)
     x, y, w = randn(g, 9, 777), randn(g, 9, 777), randn(g, 777)
