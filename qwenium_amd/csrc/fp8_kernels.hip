@@ -124,8 +124,12 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
     const int64_t blocks = rows * ((cols + kFp8Block - 1) / kFp8Block);
     if (blocks <= 0) return hipSuccess;
     if (blocks > (1ll << 28) - 16) return hipErrorInvalidValue;  // (16 threads each in whole workgroups of 256, below 2^32 a launch)
-    // nt: rows of whole lines, more than an L2 holds, past the caches (32768 x 512 x 2 f32 28.2 -> 27.4 us)
-    const bool whole = cols % 8 == 0, nt = cols % kFp8Block == 0 && rows * cols > kL2Bytes;
+    // nt: rows of whole lines past the caches where they are more than an L2 holds and fewer than eight do (32768 x 512 SwiGLU
+    // bf16 21.7 -> 20.0 us, f32 without 9.6 -> 9.2).  With the product that reads them next the two are level, us through /
+    // past: 8 MB 91.5 / 91.4, 101 / 100, 12 MB 147 / 146, 17 MB 130 / 131, 128 / 127, 119 / 119 (once 108 / 114); beyond,
+    // 34 MB 229 / 231, 232 / 236.
+    const int64_t bytes = rows * cols;
+    const bool whole = cols % 8 == 0, nt = cols % kFp8Block == 0 && bytes > kL2Bytes && bytes < 8 * kL2Bytes;
     const dim3 grid((unsigned)((blocks + 15) / 16));
 #define QMOE_Q8A(B, V, A) \
     hipLaunchKernelGGL((k_fp8_quantize<B, V, A>), grid, dim3(256), 0, stream, x, (uint32_t)blocks, cols, q, scale, nt)
@@ -713,15 +717,15 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     p.NB = (p.N + kFp8Block - 1) / kFp8Block;
     // Workgroups of rows x cols tiles (grouped: at most).
     auto wgs = [&](int rows, int cols) { return fp8_max_tiles(p, rows) * ((p.N + cols - 1) / cols); };
-    // Results past the caches where they are larger than an L2 (4 MB; one matrix, whose weights stay in the caches: than
-    // eight) and their rows whole lines, us without / with: 256 experts of 1024 x 2048, 8192 rows 96 / 88, 32768 141 /
-    // 132, f32 188 / 185, 1688 rows of 2816 x 704 f32 56 / 53, 8192 x 4096 x 4096 125 / 121, f32 220 / 216; 64 rows an
-    // expert (1 MB) 69 / 72.  Rows that share lines: bf16 of experts 8192 x 1000 96 / 91, 32768 139 / 137, but f32
-    // 185 / 190 and one matrix 8192 x 4001 79 / 91.  (What reads them next is no slower.)
+    // Results of experts past the caches where they are larger than an L2 (4 MB) and below 64 MB, in whole lines or bf16 of
+    // few rows an expert: the product and what reads it next (the block's quantization or weighted sum), us through /
+    // past; 256 experts of 1024 x 2048 and 2048 x 512 bf16, 8 MB 95 / 93, 17 MB 111 / 105, 34 MB 67 / 63, 67 MB 203 / 205
+    // and 94 / 93, 134 MB 132 / 136; f32 17 MB 101 / 95, 34 MB 64 / 60, 49 MB 133 / 127, 98 MB 86 / 88, 185 MB 159 / 165;
+    // rows that share lines (992 columns) 16 MB 111 / 105, 33 MB 139 / 135.  One matrix: 34 MB 118 / 118, 67 MB 232 / 234.
     const int elem = bf16 ? 2 : 4;
+    const int64_t out_bytes = (int64_t)p.R * p.N * elem;
     const bool whole_lines = p.N * elem % 128 == 0 && (uintptr_t)p.y % 128 == 0;
-    p.stream_out = (int64_t)p.R * p.N * elem > (p.offsets ? kL2Bytes : 8 * kL2Bytes) &&
-                   (whole_lines || (p.offsets && bf16 && p.R / p.E <= 256));
+    p.stream_out = p.offsets && out_bytes > kL2Bytes && out_bytes < 16 * kL2Bytes && (whole_lines || (bf16 && p.R / p.E <= 256));
     // A grid of at most two workgroups per CU that streams its operands once: latency.
     if (wgs(p.offsets ? 16 : 32, 16) <= 2 * kFp8Cus)
         return p.offsets || p.R <= 16 ? launch_stream<1, 4>(p, bf16, stream) : launch_stream<2, 2>(p, bf16, stream);

@@ -137,8 +137,11 @@ hipError_t launch_residual_norm(ResidualNorm p, bool bf16, int n_tokens, hipStre
     if (n_tokens <= 0) return hipSuccess;
     if (p.H > 16384) return hipErrorInvalidValue;
     const bool whole = p.H % 8 == 0;
-    // rows of whole lines, more than an L2 holds: past the caches (4096 x 2816 bf16 25.4 -> 24.2 us, without a gate 18.8 -> 17.9)
-    p.stream_out = p.H % kFp8Block == 0 && (int64_t)n_tokens * p.H * 2 > kL2Bytes;
+    // Rows of whole lines past the caches where they are more than an L2 holds and fewer than eight do (of two bytes a
+    // column; 4096 x 2816 bf16 25.4 -> 24.2 us).  With the product that reads them next, us through / past: 2048 x 2048 bf16
+    // 138 / 134, 4096 201 / 199, 2048 x 4096 99 / 97, 1500 x 2048 f32 129 / 126; beyond, 8192 x 2048 343 / 347, with a norm 38 / 39.
+    const int64_t bytes = (int64_t)n_tokens * p.H * 2;
+    p.stream_out = p.H % kFp8Block == 0 && bytes > kL2Bytes && bytes < 8 * kL2Bytes;
     if (bf16) { if (whole) launch_norm<true, true>(p, n_tokens, stream); else launch_norm<true, false>(p, n_tokens, stream); }
     else { if (whole) launch_norm<false, true>(p, n_tokens, stream); else launch_norm<false, false>(p, n_tokens, stream); }
     return hipGetLastError();

@@ -194,13 +194,14 @@ static void row_grid(int n_tokens, int64_t pieces, dim3& grid, dim3& block) {
 // Rows to the experts' order: a token's workgroups read its row once and write it
 // top_k times (reading by sorted row would read it top_k times).  Rows behind the
 // last expert's belong to no token: zeros, by the token with those list indices.
-// 4096 rows of 4 KB, 8 times (151 MB): 27 us, 5.6 TB/s.  A thread takes 16 bytes; a
+// 4096 rows of 4 KB, 8 times (151 MB): 24 us, 6.3 TB/s.  A thread takes 16 bytes; a
 // row's last 16 may overlap the ones before (the same bytes written twice).  V: 16 bytes, or
-// single bytes for rows shorter than that.  NT: past the caches, where the rows are more
-// than these hold (8192 x 2 rows of 8 KB 40 -> 31 us).
+// single bytes for rows shorter than that.  Written through the caches: past them
+// what reads the rows next pays (with a quantization of them, us through / past: 67 MB
+// 39 / 42, 134 MB 71 / 78, 268 MB 145 / 155, f32 185 MB 65 / 76).
 // ---------------------------------------------------------------------------
 typedef uint32_t u32x4a1 __attribute__((ext_vector_type(4), aligned(1)));
-template <typename V, bool NT>
+template <typename V>
 __global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int bytes, int top_k, int R, const int32_t* total,
                                                        const int32_t* place, uint8_t* y) {
     constexpr int kSize = sizeof(V);
@@ -214,10 +215,7 @@ __global__ __launch_bounds__(256) void k_gather_tokens(const uint8_t* x, int byt
 #pragma unroll 4
     for (int j = 0; j < top_k; ++j) {
         const int p = pl[j];
-        if (p >= 0 && p < R) {
-            if constexpr (NT) __builtin_nontemporal_store(v, (V*)(y + (uint64_t)p * bytes + i));
-            else *(V*)(y + (uint64_t)p * bytes + i) = v;
-        }
+        if (p >= 0 && p < R) *(V*)(y + (uint64_t)p * bytes + i) = v;
         const int r = t * top_k + j;
         if (r >= last) *(V*)(y + (uint64_t)r * bytes + i) = V{};
     }
@@ -230,13 +228,11 @@ hipError_t launch_gather_tokens(const void* x, int elem, int n_tokens, int n_col
     dim3 grid, block;
     row_grid(n_tokens, bytes >= 16 ? (bytes + 15) / 16 : bytes, grid, block);
     if (grid.y > 65535) return hipErrorInvalidValue;
-    const bool stream_out = (int64_t)n_tokens * top_k * bytes > 8 * kL2Bytes;
-#define QMOE_GATHER(...)                                                                                               \
-    hipLaunchKernelGGL((k_gather_tokens<__VA_ARGS__>), grid, block, 0, stream, (const uint8_t*)x, bytes, top_k,        \
+#define QMOE_GATHER(V)                                                                                                 \
+    hipLaunchKernelGGL((k_gather_tokens<V>), grid, block, 0, stream, (const uint8_t*)x, bytes, top_k,        \
                        n_tokens * top_k, total, place, (uint8_t*)y)
-    if (bytes < 16) QMOE_GATHER(uint8_t, false);
-    else if (stream_out) QMOE_GATHER(u32x4a1, true);
-    else QMOE_GATHER(u32x4a1, false);
+    if (bytes < 16) QMOE_GATHER(uint8_t);
+    else QMOE_GATHER(u32x4a1);
 #undef QMOE_GATHER
     return hipGetLastError();
 }
@@ -269,12 +265,10 @@ struct Piece {
         }
     }
     // the columns from c + skip on
-    template <bool WHOLE, bool NT = false>
+    template <bool WHOLE>
     __device__ __forceinline__ void store(void* row, int c, int H, int skip) const {
         if (WHOLE || (H >= C && skip == 0)) {
-            u32x4a2* p = (u32x4a2*)((uint8_t*)row + (int64_t)c * (16 / C));
-            if constexpr (NT) __builtin_nontemporal_store(r, p);
-            else *p = r;
+            *(u32x4a2*)((uint8_t*)row + (int64_t)c * (16 / C)) = r;
         } else {
 #pragma unroll
             for (int i = 0; i < C; ++i)
@@ -369,10 +363,11 @@ hipError_t launch_combine_tokens(const void* ys, bool bf16, int n_tokens, int H,
 // dw[t][j] = <dy[t], ys[place[t][j]]>.  One workgroup per token, so no sum is
 // shared between workgroups: a thread adds its columns' products in turn (16 bytes of 8
 // assignments in flight), then the tree over its wave's lanes and the waves in turn.
-// Rows behind the last expert's get zeros.  4096 x 8 rows of 4 KB (285 MB) 61.5 us, 4.6
-// TB/s; 8192 x 2 of 8 KB 85 (96 through the caches).
+// Rows behind the last expert's get zeros.  Written through the caches, as the gather's
+// (with a quantization of dys, us through / past: 67 MB 56 / 60, 134 MB 98 / 112, f32 185
+// MB 105 / 121).  4096 x 8 rows of 4 KB (285 MB) 52 us, 5.5 TB/s; 8192 x 2 of 8 KB 85.
 // ---------------------------------------------------------------------------
-template <bool BF16, bool WHOLE, bool NT>
+template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, const void* ys, int H, int top_k, int R,
                                                              const int32_t* total, const int32_t* place, const float* w,
                                                              void* dys, float* dw) {
@@ -412,14 +407,14 @@ __global__ __launch_bounds__(1024) void k_combine_tokens_bwd(const void* dy, con
                         o[i] = wj[j] * g[i];
                     }
                     out.set(o);
-                    out.template store<WHOLE, NT>(row_at<BF16>(dys, p[j], H), c, H, c0 - c);
+                    out.template store<WHOLE>(row_at<BF16>(dys, p[j], H), c, H, c0 - c);
                 }
                 const int a = t * top_k + j0 + j;
                 if (a >= last) {
 #pragma unroll
                     for (int i = 0; i < C; ++i) o[i] = 0.0f;
                     out.set(o);
-                    out.template store<WHOLE, NT>(row_at<BF16>(dys, a, H), c, H, c0 - c);
+                    out.template store<WHOLE>(row_at<BF16>(dys, a, H), c, H, c0 - c);
                 }
             }
         }
@@ -444,16 +439,14 @@ hipError_t launch_combine_tokens_bwd(const void* dy, const void* ys, bool bf16, 
                                      hipStream_t stream) {
     if (n_tokens <= 0) return hipSuccess;
     const int C = bf16 ? 8 : 4;
-    const bool whole = H % C == 0, stream_out = (int64_t)n_tokens * top_k * H * (16 / C) > 8 * kL2Bytes;
+    const bool whole = H % C == 0;
     const int64_t pieces = ((int64_t)H + C - 1) / C;
     const dim3 grid(n_tokens), block((unsigned)(pieces < 1024 ? (pieces + 63) / 64 * 64 : 1024));
-#define QMOE_BWD(...)                                                                                                  \
-    hipLaunchKernelGGL((k_combine_tokens_bwd<__VA_ARGS__>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, \
+#define QMOE_BWD(B, V)                                                                                                 \
+    hipLaunchKernelGGL((k_combine_tokens_bwd<B, V>), grid, block, 0, stream, dy, ys, H, top_k, n_tokens * top_k, total, \
                        place, w, dys, dw)
-#define QMOE_BWD_NT(B, V) do { if (stream_out) QMOE_BWD(B, V, true); else QMOE_BWD(B, V, false); } while (0)
-    if (bf16) { if (whole) QMOE_BWD_NT(true, true); else QMOE_BWD_NT(true, false); }
-    else { if (whole) QMOE_BWD_NT(false, true); else QMOE_BWD_NT(false, false); }
-#undef QMOE_BWD_NT
+    if (bf16) { if (whole) QMOE_BWD(true, true); else QMOE_BWD(true, false); }
+    else { if (whole) QMOE_BWD(false, true); else QMOE_BWD(false, false); }
 #undef QMOE_BWD
     return hipGetLastError();
 }
