@@ -608,6 +608,54 @@ def test_matmul_large_products_that_cancel(gpu, E, R, N, K, dtype):
     assert torch.equal(y, want)
 
 
+# tile, experts (0: dense), rows, n, k, rows an expert: many steps of 128 columns through each tile's buffers, their number
+# a multiple of 4 (row scales in 16 bytes) and not, k whole blocks (weights of one row tile past the caches) and not
+STEADY = [("256x256", 0, 4100, 4104, 1040, ""), ("256x256", 0, 4100, 4104, 1024, ""), ("256x256", 0, 4096, 4096, 2048, ""),
+          ("128x256", 0, 2050, 4100, 1040, ""), ("128x256", 0, 2050, 4100, 1024, ""), ("64x128", 0, 1000, 2600, 1040, ""),
+          ("64x128", 0, 1000, 2600, 1536, ""), ("32x128", 0, 600, 2100, 1040, ""), ("32x128", 0, 600, 2100, 2048, ""),
+          ("256x256", 8, 10000, 2100, 1040, "any"), ("256x256", 8, 10000, 2100, 1536, "any"), ("256x256", 16, 3600, 5000, 1024, "any"),
+          ("256x256", 16, 3600, 5000, 1152, "even"), ("160x128", 40, 5200, 1000, 1024, "even"), ("160x128", 40, 5200, 1000, 1040, "any"),
+          ("160x128", 40, 5200, 1000, 1152, "any"), ("128x128", 20, 1600, 2000, 1024, "even"), ("128x128", 20, 1600, 2000, 1040, "any"),
+          ("64x128", 40, 1400, 1000, 1024, "even"), ("64x128", 40, 1400, 1000, 1040, "any"), ("64x128, two buffers", 40, 1400, 1000, 512, "any"),
+          ("32x64, four buffers", 300, 2400, 260, 1024, "any"), ("32x64, four buffers", 300, 2400, 260, 2064, "any"),
+          ("32x64, three buffers", 40, 500, 1000, 896, "any")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tile,E,R,N,K,cuts", STEADY, ids=["-".join(map(str, c)) for c in STEADY])
+def test_matmul_tiles_over_many_steps(gpu, tile, E, R, N, K, cuts, dtype):
+    """Against 64 bits on the device, the whole result, with f32 sums for either type (check_product's roundings without
+    its allowance for the e4m3 instruction).  Uneven experts hold few rows, none, and more than a tile's, so that waves
+    of a workgroup make different numbers of subtiles."""
+    g = gen(R + N + K)
+    a, s = (t.to(gpu) for t in fp8_rows(g, R, K))
+    w, sw = (t.to(gpu) for t in fp8_weights(g, max(E, 1), N, K))
+    rows = torch.randperm(R, generator=g).to(torch.int32)
+    rows[R // 2] = R
+    bounds, kw = [0, R], {}
+    if E:
+        cut = torch.linspace(0, R, E + 1).int()[1:-1] if cuts == "even" else \
+            torch.sort(torch.randint(0, R, (E - 1,), generator=g)).values.int()
+        bounds = [0] + cut.tolist() + [R]
+        kw["offsets"] = torch.tensor(bounds, dtype=torch.int32, device=gpu)
+    else:
+        w, sw = w[0], sw[0]
+    y = qa.fp8_matmul(a, s, w, sw, rows=rows.to(gpu), out_dtype=dtype, **kw)
+    assert torch.equal(y, qa.fp8_matmul(a, s, w, sw, rows=rows.to(gpu), out_dtype=dtype, **kw))
+    y = y.double()
+    at = rows.long().to(gpu)
+    A = whole(a.float(), s)[at % R] * (at < R)[:, None]
+    loss = (2 * 128 + blocks(K) + 8) * U32
+    for e in range(max(E, 1)):
+        i, j = bounds[e], bounds[e + 1]
+        if j > i:
+            W = whole((w[e] if E else w).float(), sw[e] if E else sw, 128)
+            want = A[i:j] @ W.T
+            off = (y[i:j] - want).abs() - loss * (A[i:j].abs() @ W.abs().T) * (1 + 2.0 ** -8) - U[dtype] * want.abs()
+            assert off.max() <= 0, f"{tile}, expert {e}: {off.max().item():.3e} over its tolerance"
+
+
 @pytest.mark.gpu
 def test_matmul_beyond_32_bit_offsets(gpu):
     """Rows, experts and outputs whose byte offsets pass 2^32."""
