@@ -14,6 +14,9 @@ block of 128 x 128; the layers of moe.py take GGUF Q4_0/Q8_0.  One block is
 Rows are torch.float32 or torch.bfloat16.  As with moe.py, work goes to the given
 stream or the current stream of the operands' device, outputs are allocated on it,
 strided rows are copied first, and wrong arguments raise ValueError before a launch.
+The calls stand outside autograd: none records a gradient (gather_tokens_backward and
+combine_tokens_backward are called by the training program), and an operand that requires
+grad is refused unless gradients are off (torch.no_grad()).
 """
 from __future__ import annotations
 
@@ -42,8 +45,16 @@ def _want(name: str, what: str, got) -> ValueError:
     return ValueError(f"{name} expected {what}, got {_describe(got)}")
 
 
+def _no_grad(name: str) -> None:
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} expected a tensor outside autograd (detach() it, or call within torch.no_grad()), "
+                         "got one that requires grad")
+
+
 def _rows(name: str, t, device=None, shape=None, dtype=None) -> torch.Tensor:
     """A read-only cuda [R, C] operand, made contiguous."""
+    if getattr(t, "requires_grad", False):
+        _no_grad(name)
     if (not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_cuda
             or (t.dtype not in _TYPES if dtype is None else t.dtype != dtype)
             or (device is not None and t.device != device) or (shape is not None and t.shape != shape)):
@@ -55,6 +66,8 @@ def _rows(name: str, t, device=None, shape=None, dtype=None) -> torch.Tensor:
 
 def _kept(name: str, t, device, shape, dtype) -> torch.Tensor:
     """An operand or output that is used in place: contiguous as it is."""
+    if getattr(t, "requires_grad", False):
+        _no_grad(name)
     if (not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device
             or not t.is_contiguous()):
         raise _want(name, f"a contiguous {str(dtype).replace('torch.', '')} {list(shape)} tensor on {device}", t)

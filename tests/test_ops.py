@@ -269,6 +269,56 @@ def test_python_refuses_host_tensors():
         qa.residual_norm(x, x, None, 1e-6)
 
 
+GRAD_CALLS = {
+    "fp8_quantize": lambda x, y, w: qa.fp8_quantize(x),
+    "gather_tokens": lambda x, y, w: qa.gather_tokens(x, None),
+    "combine_tokens": lambda x, y, w: qa.combine_tokens(x, None, w),
+    "gather_tokens_backward": lambda x, y, w: qa.gather_tokens_backward(x, None),
+    "combine_tokens_backward": lambda x, y, w: qa.combine_tokens_backward(y, x, None, w),
+    "residual_norm": lambda x, y, w: qa.residual_norm(x, y, w, 1e-6),
+}  # (fp8_matmul's first operand is e4m3: on the device, below)
+
+
+@pytest.mark.parametrize("name", GRAD_CALLS)
+def test_operands_that_require_grad_are_refused(name):
+    """No call records a gradient: an operand that asks for one is refused rather than its gradient lost."""
+    x, y, w = torch.zeros(4, 128, requires_grad=True), torch.zeros(4, 128), torch.zeros(128)
+    with pytest.raises(ValueError, match="(x|ys) expected a tensor outside autograd .* requires grad"):
+        GRAD_CALLS[name](x, y, w)
+    with torch.no_grad(), pytest.raises(ValueError, match="expected a cuda"):
+        GRAD_CALLS[name](x, y, w)
+
+
+@pytest.mark.gpu
+def test_operands_that_require_grad_on_device(gpu):
+    """Every operand that a gradient could be asked of; within no_grad the calls run and give what they gave."""
+    g = gen(8)
+    T, k, E, H = 6, 2, 4, 128
+    x, ys, w = randn(g, T, H).to(gpu), randn(g, T * k, H).to(gpu), torch.rand(T, k, generator=g).to(gpu)
+    o = device_order(gpu, routing(g, T, E, k), E)
+    q, s = qa.fp8_quantize(x)
+    m, sm = (t.to(gpu) for t in fp8_weights(g, 64, H))
+    vec = torch.rand(H, generator=g).to(gpu)
+    for call, args in ((lambda a: qa.gather_tokens(a, o), (x,)), (lambda a, b: qa.combine_tokens(a, o, b), (ys, w)),
+                       (lambda a, b, c: qa.combine_tokens(a, o, b, residual=c), (ys, w, x)),
+                       (lambda a: qa.gather_tokens_backward(a, o), (ys,)),
+                       (lambda a, b, c: qa.combine_tokens_backward(a, b, o, c)[0], (x, ys, w)),
+                       (lambda a: qa.fp8_quantize(a)[1], (x,)), (lambda a, b: qa.fp8_matmul(q, a, m, b), (s, sm)),
+                       (lambda a, b, c: qa.residual_norm(a, b, c, 1e-6).h, (x, x.clone(), vec)),
+                       (lambda a, b, c: qa.residual_norm(x, x.clone(), None, 1e-6, post_w=a, scale=b, gate=c, gate_act="silu").h,
+                        (vec, vec.clone(), x.clone()))):
+        want = call(*args)
+        assert not want.requires_grad
+        for i in range(len(args)):
+            asks = [a.detach().clone().requires_grad_(j == i) for j, a in enumerate(args)]
+            with pytest.raises(ValueError, match="outside autograd"):
+                call(*asks)
+            with torch.no_grad():
+                assert torch.equal(call(*asks), want)
+            with torch.inference_mode():
+                assert torch.equal(call(*asks), want)
+
+
 @pytest.mark.gpu
 def test_python_refusals_on_device(gpu):
     x = torch.zeros(4, 128, device=gpu)
