@@ -375,8 +375,10 @@ int qmoe_fp8_quantize(const void* x, int32_t x_type, int32_t n_rows, int32_t n_c
  *   rows NULL: s = r (n_rows == a_rows); else s = rows[r], and a row with s outside
  *     [0, a_rows) is zeros.
  * k is a multiple of 16; a and w are 16-byte aligned; n_rows <= 2^30, n_experts <=
- * 1024, and the rows' and columns' tiles fit one launch (below 2^32 threads).  y overlaps no input.  Offsets that fall give rows of more than one expert
- * either one's values. */
+ * 1024, and the rows' and columns' tiles fit one launch (below 2^32 threads).  y overlaps
+ * no input.  Offsets that fall are followed within the bounds, but a row of theirs may hold
+ * any of its experts' values or what it held.  The product of two scales is formed in f32:
+ * below 2^-126 it loses bits, above f32's largest number it is infinite. */
 int qmoe_fp8_matmul(const uint8_t* a, const float* a_scale, int32_t a_rows, const uint8_t* w, const float* w_scale,
                     int32_t n_experts, int32_t n, int32_t k, const int32_t* offsets, const int32_t* rows,
                     int32_t n_rows, void* y, int32_t y_type, void* hip_stream);

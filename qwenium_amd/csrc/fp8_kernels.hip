@@ -408,10 +408,11 @@ struct Fp8Tile {
 };
 
 // Many rows: a workgroup of WM x WN waves makes a tile of 16 MS WM rows and 16 NS WN
-// columns.  Each step of 128 columns of K comes straight to LDS (ST buffers): rows of 128 bytes, whose eight 16-byte pieces lie at slots piece ^
-// (row & 7), so that the 16 rows of a fragment meet all banks (measured: no conflicts).
-// The 16-row subtiles go to the WM waves in turn and those without rows are left out
-// (MI: how many).
+// columns.  Each step of 128 columns of K comes straight to LDS (ST buffers): rows of 128
+// bytes, whose eight 16-byte pieces lie at slots piece ^ (row & 7), so that the 16 rows of a
+// fragment meet all banks.  (What conflicts there are come from the row scales, 4 bytes read
+// at steps of 16: two cycles a read, 8192 of a CU's in 8192 x 4096 x 4096.)  The 16-row
+// subtiles go to the WM waves in turn and those without rows are left out (MI: how many).
 template <int WM, int WN, int MS, int NS, int ST, bool BF16>
 __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     using T = Fp8Tile<WM, WN, MS, NS, ST, BF16>;
@@ -423,9 +424,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     n0 *= T::kBN;
     if (!fp8_find_tile(p, T::kBM, tile, e, row0, end, once)) return;
     // Weights that this row tile alone reads, in whole 128-byte lines, go past the caches.  256 experts of
-    // 1024 x 2048, four layers' weights in turn, us without and with: 80 rows 33.0 / 29.5, 512 rows 83 / 69,
-    // 4096 96 / 90, 32768 151 / 148; with two tiles an expert (128 of 1408 x 2816, 32768 rows) 225 / 266;
-    // with 5.5 lines a row (128 of 2816 x 704, 1688 rows) 58 / 64.
+    // 1024 x 2048, several layers' weights in turn, us without and with: 80 rows 28.8 / 27.2, 1024 rows 90 / 80, 4096
+    // 95 / 91, 32768 190 / 185; with two tiles an expert (80000 rows) 384 / 410; with 5.5 lines a row (128 of 2816 x
+    // 704, 1688 rows) 58 / 63, 4000 rows 65 / 70.
     once = once && p.K % kFp8Block == 0;
     const int nrows = end - row0 < T::kBM ? end - row0 : T::kBM;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
         constexpr int MI = decltype(mi_c)::value;
         constexpr int kLate = MI >= 4 ? 2 : 1;  // subtiles whose products come after the step's last row fragment is read
         // Eight waves load half of a stage after the barrier, half in the next step: all at once they hold each other up
-        // (8192 x 4096 x 4096 bf16 134 us, in halves 128, both before the stores went out in lines; tiles of four waves lose 1-2% by it).
+        // (8192 x 4096 x 4096 bf16 220 us, in halves 214; tiles of four waves lose 1-2% by it).
         constexpr int kFirst = T::kWaves == 8 && MI >= 4 ? (T::kLoads + 1) / 2 : T::kLoads;
         int buf = 0;
         float ws_next = scalar_load(sw);
@@ -636,7 +637,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tile(Fp8Product p) {
     else run(std::integral_constant<int, kQuarter>{});
 
     // Two 64-byte pieces of a row's columns: lanes of rows 8 apart swap one of theirs, so that a store covers whole
-    // 128-byte lines (256 experts x 32768 rows 136 -> 133 us, with 93 MB written for 67 before).
+    // 128-byte lines (256 experts x 32768 rows: 67 MB written for 93).
     constexpr bool kLines = NS / T::P % 2 == 0;
     const bool lines = kLines && nw0 + 16 * NS <= p.N;
 #pragma unroll
@@ -745,7 +746,9 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
     // 218 / 185 / 203 / 198 / 227, 156 rows 246 / 220 / 242 / 237 / 267, 187 rows 254 / 274 / 281 / 271 / 302; f32: 64 rows
     // 150 / 138 / 136 / 129 / 142, 128 rows 222 / 189 / 210 / 206 / 233, 187 rows 269 / 285 / 292 / 279 / 314; 128 of 1408 x
     // 2816, 125 rows 221 / 176 / 201 / 184 / 210; 128 of 2816 x 704, 62 rows 93 / 85 / 92 / 81 / 86, f32 97 / 91 / 96 / 87 /
-    // 93; 64 of 1536 x 1536, 281 rows 131 / 105 / 121 / 114 / 134; 8 of 2048 x 2048, 2000 rows 125 / 133 / 134 / 130 / 160.
+    // 93; 64 of 1536 x 1536, 281 rows 131 / 105 / 121 / 114 / 134, 562 rows 201 / 187 / 208 / 201 / 241; 500 rows of 8 of
+    // 4096 x 1024 57 / 45 / 55 / 46 / 55, of 256 of 1024 x 1024 306 / 331 / 337 / 327 / 407; 8 of 2048 x 2048, 2000 rows 125 /
+    // 133 / 134 / 130 / 160.
     if (mean >= 110) {
         if (((mean > 160 && mean <= 256) || mean >= 1024) && wgs(256, 256) >= kFp8Cus)
             return launch_tile<2, 4, 8, 4, 2>(p, bf16, stream);
@@ -754,11 +757,11 @@ hipError_t launch_fp8_matmul(Fp8Product p, bool bf16, hipStream_t stream) {
         return launch_tile<2, 2, 4, 4, 2>(p, bf16, stream);
     }
     // Weights streamed for few rows: small tiles, many loads in flight, unless K is soon over; up to 20 rows also where
-    // there would be few large tiles.  Us with 32x64 in four buffers / in three / 64x128 in three / in two: 256 experts
-    // of 1024 x 2048, 2 tokens 8.4 / 9.6 / 10.8 / 15.9, 10 tokens 24.7 / 26.1 / 27.5 / 25.6, 256 82 / 82 / 84 / 88, 512
-    // 88 / 89 / 86 / 88; 32 of 2048 x 4096, 100 tokens 48 / 53 / 57 / 61; 128 of 2816 x 704 f32, 64 tokens 52 / 50 / 52 /
-    // 52, 211 57 / 55 / 56 / 58, 500 76 / 74 / 65 / 66; 256 of 2048 x 512, 64 tokens 42 / 40 / 43 / 39, 211 53 / 48 /
-    // 50 / 47.
+    // there would be few large tiles.  Us with 32x64 in four buffers / in three / 64x128 in three / in two, bf16 (f32 within
+    // 3%): 256 experts of 1024 x 2048, 2 tokens 10.5 / 11.7 / 13.8 / 16.6, 10 tokens 28 / 29 / 32 / 29, 256 84 / 84 / 86 / 90,
+    // 512 95 / 94 / 91 / 93; 32 of 2048 x 4096, 100 tokens 54 / 57 / 61 / 64; 128 of 2816 x 704, 30 tokens 48 / 46 / 48 / 47,
+    // 64 55 / 52 / 55 / 53, 211 60 / 57 / 57 / 54, 500 82 / 78 / 63 / 63; 256 of 2048 x 768, 64 65 / 58 / 61 / 59, 211 80 / 73
+    // / 74 / 71; 64 of 3584 x 896, 100 39 / 37 / 38 / 40; 256 of 2048 x 512, 64 tokens 49 / 44 / 47 / 42, 211 61 / 54 / 56 / 51.
     if ((mean < 12 || (mean < 20 && wgs(64, 128) < 4 * kFp8Cus)) && p.KB >= 8)
         return launch_tile<1, 4, 2, 1, 4>(p, bf16, stream);
     if (mean < 16 && p.KB > 4 && p.KB < 8) return launch_tile<1, 4, 2, 1, 3>(p, bf16, stream);

@@ -141,7 +141,8 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     a [A, k], a_scale [A, ceil(k/128)] (fp8_quantize's); w [n, k], w_scale
     [ceil(n/128), ceil(k/128)].  Grouped: w [E, n, k], w_scale [E, ...] and offsets
     (int32 [E+1], a TokenOrder's): row r is multiplied by expert e's matrix for
-    offsets[e] <= r < offsets[e+1]; rows of no expert are left as they were.
+    offsets[e] <= r < offsets[e+1]; rows of no expert are left as they were (in a new
+    result: uninitialised).
     rows (int32 [R], a TokenOrder's tokens): row r is a[rows[r]]; an index outside a
     gives zeros.  out [R, n] may be given, float32 or bfloat16; else out_dtype is its type."""
     with _on(stream):
