@@ -82,6 +82,11 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+# torch.cuda.current_stream(i).cuda_stream without the Stream object around it (1.9 us of a 5 us call), and the
+# current device, by torch's own bindings where they are
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
 _NO_STREAM = contextlib.nullcontext()
 
 
@@ -93,14 +98,12 @@ def _launch(fn, device, stream, *args) -> None:
     """Calls fn(*args, stream) with the operands' device current."""
     index = device.index
     if stream is None:
-        # torch.cuda.current_stream(device).cuda_stream without the Stream object around
-        # it (1.9 us of a 5 us call)
-        handle = torch._C._cuda_getCurrentRawStream(index)
+        handle = _raw_stream(index)
     elif stream.device != device:
         raise ValueError(f"stream expected one of {device}, got one of {stream.device}")
     else:
         handle = stream.cuda_stream
-    if index == torch._C._cuda_getDevice():
+    if index == _current_device():
         rc = fn(*args, handle)
     else:
         with torch.cuda.device(device):

@@ -1164,6 +1164,27 @@ def test_other_stream_and_same_bits(gpu):
 
 
 @pytest.mark.gpu
+def test_streams_and_devices_without_torchs_bindings(gpu, monkeypatch):
+    """The stream handle is the current stream's, by either way to it; with another device current the operands' own is
+    set for the launch."""
+    from qwenium_amd import ops
+    x = randn(gen(5), 9, 300).to(gpu)
+    want = qa.fp8_quantize(x)[0].view(torch.uint8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            assert ops._raw_stream(0) == stream.cuda_stream and ops._current_device() == 0
+    monkeypatch.setattr(ops, "_raw_stream", lambda i: torch.cuda.current_stream(i).cuda_stream)
+    monkeypatch.setattr(ops, "_current_device", lambda: 1)
+    assert torch.equal(qa.fp8_quantize(x)[0].view(torch.uint8), want)
+    with torch.cuda.stream(side):
+        got = qa.fp8_quantize(x)[0].view(torch.uint8)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [3, 200])
 def test_graph_replays(gpu, T):
     """Two captured blocks, replayed in turn on changed inputs with eager work between: the eager results."""
