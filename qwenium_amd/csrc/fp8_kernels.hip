@@ -155,17 +155,18 @@ hipError_t launch_fp8_quantize(const void* x, bool bf16, int64_t rows, int cols,
 // columns to the largest, P, before they add them, and drop what lies below 2^-13 P
 // (measured, 16x16x128_f8f6f4 and 16x16x32_fp8_fp8 alike: beside P = 2^16 a product of
 // 2^3 counts and one of 2^2 is lost), so that a sum whose large terms cancel is lost
-// whole.  16x16x128_f8f6f4 has 3.4 times the f16 rate (8192 x 4096 x 4096 took 125 us by
-// it); 16x16x32_fp8_fp8 has the f16 rate.
+// whole.  16x16x128_f8f6f4 has twice the f16 rate (in registers 4.4 and 2.1-2.4 PFLOP/s;
+// 8192 x 4096 x 4096 took 125 us by it); 16x16x32_fp8_fp8 has the f16 rate.
 // The weights are the MFMA's rows and the activations its columns: a lane then
 // holds four consecutive n of one row r, whose scale is one value per lane, and
 // stores them together.  (Both operands take the same permutation of a block's
 // columns, which leaves its sum as it is: lane group g reads 16-byte pieces g and
 // g + 4.)
 //   Where the time goes (us): 8192 x 4096 x 4096 208-232 (1.2-1.3 PFLOP/s, the rate of a
-// library's bf16 product and of the f16 instruction in registers alone, 1.18), f32 results
-// 218-236; 256 experts of 1024 x 2048: 80 rows 27 (147 MB: 5.4 TB/s), 4096 rows 89 (6.0
-// TB/s), 32768 rows 185-200 (137 GFLOP: 0.7 PFLOP/s beside 613 MB).
+// library's bf16 product), f32 results 218-236: the matrix instructions are busy in 53% of
+// the cycles, and the conversions to f16 and the scales' fmas, 66000 vector instructions a
+// SIMD of 4 cycles each, take as many again beside them; 256 experts of 1024 x 2048: 80 rows
+// 26-28 (147 MB: 5.4 TB/s), 4096 rows 89 (6.0 TB/s), 32768 rows 182-200 (0.7 PFLOP/s).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
