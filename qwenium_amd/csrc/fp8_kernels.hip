@@ -26,8 +26,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 // covers 512 columns; no LDS, no barrier.  Bound by memory: 4096 x 2048 f32 (42 MB) 8.2
 // us, 5.1 TB/s (0.5 of it for the exact quotients); 32768 x 512 SwiGLU of bf16 (84 MB)
 // 18.5-19.9 us, 4.4 TB/s, level with its arithmetic (2 more with expf; 0.5 of it for the
-// blocks in f64, whose registers are kept within eight waves a SIMD); GeGLU 22.6-22.9, of
-// gates N(0, 4) 26.9, its values' own error bounds 0.8-1 of it.
+// blocks in f64, whose registers are kept within eight waves a SIMD); GeGLU 22.6-24, of
+// gates four times as wide 27-28, its values' own error bounds 0.8-1 of it.
 // ---------------------------------------------------------------------------
 // v = g sigmoid(z) u and a bound of its relative error.  sigmoid_product is off by up to 5 2^-24 (the hardware's 2^t 2, its
 // remainder 1, the quotient 1/2, the product 1).  SwiGLU's z is g; gelu's tanh form has z = 2 sqrt(2/pi) (g + 0.044715 g^3),

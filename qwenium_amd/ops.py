@@ -13,7 +13,8 @@ block of 128 x 128; the layers of moe.py take GGUF Q4_0/Q8_0.  One block is
 
 Rows are torch.float32 or torch.bfloat16.  As with moe.py, work goes to the given
 stream or the current stream of the operands' device, outputs are allocated on it,
-strided rows are copied first, and wrong arguments raise ValueError before a launch.
+strided rows are copied first, and wrong arguments raise ValueError, or QmoeError where
+the C ABI refuses them (sizes, overlapping buffers), before a launch.
 The calls stand outside autograd: none records a gradient (gather_tokens_backward and
 combine_tokens_backward are called by the training program), and an operand that requires
 grad is refused unless gradients are off (torch.no_grad()).

@@ -761,6 +761,26 @@ def test_sort_tokens(gpu, T, E, k, kind):
 
 
 @pytest.mark.gpu
+def test_sort_tokens_many(gpu):
+    """33 million assignments, a chunk of many rounds a workgroup; checked on the device."""
+    T, k, E = (1 << 23) + 5, 4, 200
+    g = torch.Generator(device=gpu).manual_seed(3)
+    idx = torch.randint(-1, E + 1, (T, k), generator=g, device=gpu, dtype=torch.int32)
+    o = qa.sort_tokens(idx, E)
+    flat = idx.view(-1)
+    valid = (flat >= 0) & (flat < E)
+    counts = torch.bincount(flat[valid].long(), minlength=E)
+    assert torch.equal(o.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+    live = int(o.offsets[E])
+    rows = o.rows[:live].long()
+    key = flat[rows].long() * (T * k) + rows
+    assert (key[1:] > key[:-1]).all() and valid[rows].all()  # by expert, ascending within one: each assignment once
+    assert (o.rows[live:] == -1).all() and (o.tokens[live:] == -1).all() and torch.equal(o.tokens[:live].long(), rows // k)
+    place = o.place.view(-1)
+    assert torch.equal(place[rows], torch.arange(live, device=gpu, dtype=torch.int32)) and (place[~valid] == -1).all()
+
+
+@pytest.mark.gpu
 def test_sort_tokens_ends(gpu):
     """No tokens: the offsets are still written.  All dropped.  A token with one expert twice."""
     o = qa.sort_tokens(torch.zeros((0, 4), dtype=torch.int32, device=gpu), 9)
@@ -1161,6 +1181,20 @@ def test_other_stream_and_same_bits(gpu):
     one = qa.combine_tokens_backward(dy, ys, o, args[8])
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(one, qa.combine_tokens_backward(dy, ys, o, args[8])))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(gpu):
+    """Blocks on two streams with nothing between them give what they give one after the other."""
+    both = [block_inputs(gen(s), 130, 512, 256, 16, 4, dt, gpu) for s, dt in ((14, torch.bfloat16), (15, torch.float32))]
+    want = [block(*args) for args in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    got = [[block(*args, stream=stream) for args, stream in zip(both, streams)] for _ in range(10)]
+    torch.cuda.synchronize()
+    for pair in got:
+        for a, b in zip(pair, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
 @pytest.mark.gpu
